@@ -118,6 +118,17 @@ std::vector<torch::Tensor> sq_dist_bwd(torch::Tensor a, torch::Tensor b, torch::
 int64_t decode_tc_error(bool reset);
 torch::Tensor decode_attention(torch::Tensor q, torch::Tensor k_cache, torch::Tensor v_cache, torch::Tensor lens,
                                double scale, int64_t splits, c10::optional<torch::Tensor> block_table);
+void paged8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Tensor vp, torch::Tensor ks, torch::Tensor vs,
+                   torch::Tensor table, torch::Tensor start, c10::optional<torch::Tensor> counts, int64_t offset);
+torch::Tensor paged8_attend(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor ks, torch::Tensor vs,
+                            torch::Tensor table, torch::Tensor lens, c10::optional<torch::Tensor> q_lens, double scale,
+                            int64_t len_add);
+void copy_pages(std::vector<torch::Tensor> pools, torch::Tensor src, torch::Tensor dst);
+torch::Tensor process_logits(torch::Tensor x, c10::optional<torch::Tensor> g, c10::optional<torch::Tensor> history,
+                             c10::optional<torch::Tensor> lens, c10::optional<torch::Tensor> prompt_lens,
+                             c10::optional<torch::Tensor> rows, c10::optional<torch::Tensor> rep, double rep0,
+                             c10::optional<torch::Tensor> pres, double pres0, c10::optional<torch::Tensor> freq, double freq0,
+                             c10::optional<torch::Tensor> bias, c10::optional<torch::Tensor> allowed);
 void fmha_fwd_peer(torch::Tensor q, torch::Tensor k, torch::Tensor v, std::vector<int64_t> peer_o,
                    std::vector<int64_t> peer_o2, int64_t sl, int64_t si, int64_t htot, int64_t h0, double scale,
                    int64_t version);
@@ -209,6 +220,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "grouped-query decode attention over a contiguous or paged (block table) KV cache", py::arg("q"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("lens"), py::arg("scale"), py::arg("splits"),
         py::arg("block_table") = py::none());
+  m.def("paged8_append", &vo::paged8_append, "bf16 rows into the pages of an e4m3 KV cache (power-of-two page scales)");
+  m.def("paged8_attend", &vo::paged8_attend, "grouped-query attention over an e4m3 paged KV cache");
+  m.def("copy_pages", &vo::copy_pages, "page copies inside pools [layers, pages, ...], one launch");
+  m.def("process_logits", &vo::process_logits, "penalties, bias and bitmask on logits, or their gradient");
   m.def("fmha_fwd_peer", &vo::fmha_fwd_peer, "Ulysses attention writing each output row to its owner rank",
         py::arg("q"), py::arg("k"), py::arg("v"), py::arg("peer_o"), py::arg("peer_o2"), py::arg("sl"), py::arg("si"),
         py::arg("htot"), py::arg("h0"), py::arg("scale"), py::arg("version") = 3);

@@ -19,11 +19,15 @@
     VO_CHECK_CUDA(x);     \
     VO_CHECK_CONTIG(x);   \
   } while (0)
+// Numbers enter error messages as text: where the C++ runtime is linked into the extension, formatting them through
+// an ostream of the host process's runtime crashes instead of raising.
+#define VO_TEXT_(x) #x
+#define VO_TEXT(x) VO_TEXT_(x)
 #define VO_CUDA_OK(call)                                                                      \
   do {                                                                                        \
     cudaError_t e_ = (call);                                                                  \
     TORCH_CHECK(e_ == cudaSuccess, "CUDA error ", cudaGetErrorString(e_), " at ", __FILE__, \
-                ":", __LINE__);                                                               \
+                ":" VO_TEXT(__LINE__));                                                             \
   } while (0)
 
 namespace vo {

@@ -28,6 +28,7 @@ from verl_omni_b200.ops import llm as LO
 from verl_omni_b200.ops.attention import attention
 from verl_omni_b200.ops import linear as L
 from verl_omni_b200.ops.decode import KVCache, PagedView, decode_attention
+from verl_omni_b200.ops.paged8 import Paged8View
 from verl_omni_b200.parallel import dist as D_
 
 
@@ -185,7 +186,8 @@ class MoEBlock(nn.Module):
         return x + part
 
     def attn(self, x, cos, sin, cache: Optional[dict], pos0: int, pos_t: Optional[torch.Tensor] = None):
-        """``pos_t`` (int64 ``[1]`` on the device, one-token steps on a :class:`KVCache`): the position comes
+        """``pos_t`` (int64 ``[1]`` on the device, one-token steps on a :class:`KVCache` or a
+        :class:`~verl_omni_b200.ops.paged8.Paged8View`, which keeps its own device positions): the position comes
         from the device, nothing is read on the host (a step that can be captured in a CUDA graph)."""
         cfg = self.cfg
         B, S, D = x.shape
@@ -197,8 +199,11 @@ class MoEBlock(nn.Module):
         k = LO.head_norm_rope(kvp, 0, cfg.kv_heads, self.k_norm, cos, sin, cfg.eps)  # [B, Hk, S, hd]
         v = kvp[..., cfg.kv_heads * hd:].view(B, S, cfg.kv_heads, hd).transpose(1, 2)
         if pos_t is not None:
+            if isinstance(cache, Paged8View) and S == 1:
+                cache.append_at(k, v)
+                return x + self.o_proj(cache.attend_at(q).reshape(B, 1, cfg.q_heads * hd))
             if not isinstance(cache, KVCache) or S != 1:
-                raise ValueError("device-position steps take one token against a contiguous KVCache")
+                raise ValueError("device-position steps take one token against a contiguous KVCache or an 8-bit paged one")
             cache.append_at(k, v, pos_t)
             o = decode_attention(q[:, :, 0], cache.k, cache.v, cache.lens_at(pos_t))  # [B, Hq, hd]
             return x + self.o_proj(o.reshape(B, 1, cfg.q_heads * hd))
@@ -211,6 +216,13 @@ class MoEBlock(nn.Module):
                 return x + self.o_proj(o.reshape(B, 1, cfg.q_heads * hd))
             if not first:
                 k, v = cache.k[:, :, :cache.len], cache.v[:, :, :cache.len]
+        elif isinstance(cache, Paged8View):
+            # 8-bit paged cache: the first rows attend to themselves in bf16, later ones (one token or a chunk, causal
+            # among themselves) to the cached codes
+            first = cache.len == 0
+            cache.append(k, v)
+            if not first:
+                return x + self.o_proj(cache.attend(q).reshape(B, S, cfg.q_heads * hd))
         elif isinstance(cache, PagedView):
             # paged cache (block pool + block table): same steps through the block-table decode kernel
             first = cache.len == 0

@@ -76,7 +76,9 @@ def build_omni_trainer(config):
         tp_group=tp_group, seed=int(config.data.seed), micro_batch_size=int(act.ppo_micro_batch_size_per_gpu),
         temperature=float(ro.temperature), kv_block_size=int(ro.kv_block_size),
         total_steps=int(config.trainer.total_training_steps), pp_size=pp, rollout_tp_group=rollout_tp_group,
-        model_path=arc.model.get("path", None))
+        model_path=arc.model.get("path", None),
+        rollout_kw=dict(kv_cache_dtype=str(ro.kv_cache_dtype), repetition_penalty=float(ro.repetition_penalty),
+                        presence_penalty=float(ro.presence_penalty), frequency_penalty=float(ro.frequency_penalty)))
     trainer.prompts_per_rank = gbs // dp
     files = config.data.get("train_files", None)
     if files:

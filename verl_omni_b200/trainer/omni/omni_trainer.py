@@ -33,10 +33,14 @@ class OmniGRPOTrainer:
                  prompt_text: int = 16, audio_tokens: int = 4, image_tokens: int = 4, response_len: int = 8,
                  loss_mode: str = "grpo", ep_group=None, tp_group=None, seed: int = 0,
                  micro_batch_size: Optional[int] = None, temperature: float = 1.0, kv_block_size: int = 0,
-                 total_steps: int = 1000, pp_size: int = 1, rollout_tp_group=None, model_path: Optional[str] = None):
+                 total_steps: int = 1000, pp_size: int = 1, rollout_tp_group=None, model_path: Optional[str] = None,
+                 rollout_kw: Optional[dict] = None):
         """``pp_size > 1``: pipeline parallelism over ``pp_size`` stages (rank r is stage r // (world / pp) of
         data-parallel rank r % (world / pp)); each stage holds a contiguous slice of the layers, the rollout
-        decodes through the stages and the update runs the 1F1B schedule over the micro-batches."""
+        decodes through the stages and the update runs the 1F1B schedule over the micro-batches.
+
+        ``rollout_kw``: further options of :class:`~verl_omni_b200.workers.rollout.llm_rollout.LLMRolloutEngine` (8-bit KV
+        cache, penalties)."""
         torch.manual_seed(seed)
         self.pp_size = int(pp_size)
         if self.pp_size > 1 and tp_group is not None and D.world_size(tp_group) > 1:
@@ -111,7 +115,7 @@ class OmniGRPOTrainer:
                 else TPContext(rollout_tp_group)
         self.rollout = LLMRolloutEngine(self.model, max_new_tokens=response_len, device=device,
                                         temperature=temperature, kv_block_size=kv_block_size, pp=self.pp,
-                                        tp=rtp)
+                                        tp=rtp, **(rollout_kw or {}))
         self.temperature = temperature
         self.loss_fn = get_omni_loss_fn(loss_mode)
         self.loss_mode = loss_mode
@@ -170,7 +174,7 @@ class OmniGRPOTrainer:
         timing = {}
         prompts = self.make_prompts(num_prompts, seed=1000 * self.step_count + self.dp_rank).repeat(self.n)
         tg = time.perf_counter()
-        out = self.rollout.generate(prompts, seed=self.step_count)
+        out = self.rollout.generate(prompts, seed=self.step_count, group=self.n)
         rewards = hash_token_reward(out, seed=7).to(self.device)
         adv = group_normalize(rewards, out.non_tensor_batch["uid"], global_std=False)
         mask = out.batch["response_mask"].to(self.device)
@@ -262,7 +266,7 @@ class OmniGRPOTrainer:
         link = self.pp
         prompts = self.make_prompts(num_prompts, seed=1000 * self.step_count + self.dp_rank).repeat(self.n)
         tg = time.perf_counter()
-        out = self.rollout.generate(prompts, seed=self.step_count)
+        out = self.rollout.generate(prompts, seed=self.step_count, group=self.n)
         rewards = hash_token_reward(out, seed=7).to(self.device)
         adv = group_normalize(rewards, out.non_tensor_batch["uid"], global_std=False)
         mask = out.batch["response_mask"].to(self.device)

@@ -3,19 +3,22 @@
 
 Batched prefill of the (multimodal) prompts, then token-by-token decode against preallocated per-layer KV
 caches (grouped-query decode kernel); sampling with temperature / top-k / top-p on the device from a
-seeded generator; returns the response ids, their log-probs under the sampling distribution
+seeded generator, after optional penalties for repeated tokens, a bias and a grammar bitmask on the logits
+(:func:`~verl_omni_b200.ops.logits.process_logits`); returns the response ids, their log-probs under the sampling distribution
 (``rollout_log_probs``) and an EOS-aware response mask.
 """
 
 from __future__ import annotations
 
 import os
-from typing import Optional
+from typing import Callable, Optional
 
 import torch
 
 from verl_omni_b200.models.moe_llm import MoELLM
 from verl_omni_b200.ops.decode import KVCache, PagedKVCache, sample_tokens
+from verl_omni_b200.ops.logits import process_logits
+from verl_omni_b200.ops.paged8 import Paged8View, PagedKVCache8
 from verl_omni_b200.utils.dataproto import DataProto
 
 
@@ -37,12 +40,12 @@ def sample_next(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
 
 
 def _graph_ok(module: MoELLM, caches, dev) -> bool:
-    """CUDA-graph decode applies to contiguous caches on a GPU.  With experts sharded over ranks the step holds
+    """CUDA-graph decode applies to contiguous and 8-bit paged caches on a GPU.  With experts sharded over ranks the step holds
     collectives; those are captured only on request (``VO_DECODE_GRAPH_EP=1``), since every rank of the group
     must then replay in step."""
     if os.environ.get("VO_DECODE_GRAPH", "1") == "0" or torch.device(dev).type != "cuda":
         return False
-    if not all(isinstance(c, KVCache) for c in caches):
+    if not all(isinstance(c, (KVCache, Paged8View)) for c in caches):
         return False
     ep = getattr(module, "ep", None)
     if ep is not None and getattr(ep, "ep", 1) > 1 and os.environ.get("VO_DECODE_GRAPH_EP", "0") != "1":
@@ -76,6 +79,11 @@ class _DecodeStep:
 
         self.ids.copy_(nxt.view(-1, 1))
         self.pos.fill_(pos)
+        paged = isinstance(self.caches[0], Paged8View)
+        if paged:
+            batch = self.caches[0].batch
+            off = self.caches[0].off
+            batch.at(off)  # the sequences' own positions
         self.calls += 1
         if self.graph is None and self.calls == 1:
             out = self._run()
@@ -93,17 +101,44 @@ class _DecodeStep:
             ext().count_launches(self.launches)
             out = self.out
         for c in self.caches:
-            c.len = pos + 1
+            if paged:
+                c.off = off + 1
+            else:
+                c.len = pos + 1
         return out
 
 
 class LLMRolloutEngine:
     def __init__(self, module: MoELLM, *, max_new_tokens: int = 256, temperature: float = 1.0, top_k: int = 0,
                  top_p: float = 1.0, eos_id: Optional[int] = None, device=None, kv_block_size: int = 0,
-                 pp=None, tp=None):
+                 pp=None, tp=None, kv_cache_dtype: str = "auto", repetition_penalty: float = 1.0,
+                 presence_penalty: float = 0.0, frequency_penalty: float = 0.0,
+                 logit_bias: Optional[torch.Tensor] = None,
+                 allowed_tokens: Optional[Callable[[torch.Tensor], Optional[torch.Tensor]]] = None):
         """``pp``: a :class:`~verl_omni_b200.parallel.pipeline.PipeLink` when ``module`` is one pipeline stage
         (:class:`~verl_omni_b200.models.moe_llm.MoEStage`): every step's hidden states travel down the stages
-        and the last stage's sampled tokens are broadcast back."""
+        and the last stage's sampled tokens are broadcast back.
+
+        ``kv_cache_dtype="fp8_e4m3"``: 8-bit paged KV cache (:class:`~verl_omni_b200.ops.paged8.PagedKVCache8`, pages of
+        ``kv_block_size`` or 64 rows); with ``generate(group=n)`` the ``n`` samples of a prompt share its pages.
+        ``repetition_penalty`` (tokens of prompt and response), ``presence_penalty`` / ``frequency_penalty`` (tokens of
+        the response), ``logit_bias`` (fp32 ``[vocab]``) and ``allowed_tokens`` (called with the response ids so far
+        ``[B, t]``, returns an int32 bitmask ``[B or 1, ceil(vocab / 32)]`` or None) shape the distribution that tokens are
+        drawn from; the returned log-probs are those of that distribution."""
+        if kv_cache_dtype not in ("auto", "fp8_e4m3"):
+            raise ValueError(f"unknown kv_cache_dtype {kv_cache_dtype!r}: auto or fp8_e4m3")
+        shaped = (repetition_penalty != 1.0 or presence_penalty or frequency_penalty or logit_bias is not None
+                  or allowed_tokens is not None)
+        if repetition_penalty <= 0:
+            raise ValueError("repetition_penalty is positive")
+        if pp is not None and (kv_cache_dtype != "auto" or shaped):
+            raise ValueError("the 8-bit KV cache and logits processing are not combined with pipeline stages")
+        if tp is not None and tp.world > 1 and kv_cache_dtype != "auto":
+            raise ValueError("the 8-bit KV cache is not combined with a tensor-parallel rollout")
+        self.kv8 = kv_cache_dtype == "fp8_e4m3"
+        self.shaping = dict(repetition=float(repetition_penalty), presence=float(presence_penalty),
+                            frequency=float(frequency_penalty), bias=logit_bias) if shaped else None
+        self.allowed_tokens = allowed_tokens
         self.module = module
         self.pp = pp
         # ``tp``: a TPContext -- tensor-parallel decode (vLLM's rollout tensor_model_parallel_size): the ranks of
@@ -116,7 +151,9 @@ class LLMRolloutEngine:
         self.device = device
 
     @torch.no_grad()
-    def generate(self, batch: DataProto, seed: int = 0) -> DataProto:
+    def generate(self, batch: DataProto, seed: int = 0, group: int = 1) -> DataProto:
+        """``group``: every ``group`` consecutive rows of the batch are the same prompt.  With the 8-bit cache it is
+        prefilled once and its pages are shared (the partly filled last one copied); otherwise it changes nothing."""
         if self.pp is not None:
             return self._generate_pp(batch, seed)
         tp = self.tp
@@ -133,7 +170,9 @@ class LLMRolloutEngine:
         dev = ids.device
         g = torch.Generator(device=dev).manual_seed(int(seed))  # sampling stays on the device
         cfg = self.module.cfg
-        if tp is not None:
+        if self.kv8:
+            caches, logits = self._prefill8(ids, af, ip, group)
+        elif tp is not None:
             caches = [KVCache(B, cfg.kv_heads // tp.world, P + self.max_new_tokens, cfg.head_dim, dev,
                               self.module.embed.dtype) for _ in self.module.layers]
         elif self.kv_block_size > 0:
@@ -147,10 +186,17 @@ class LLMRolloutEngine:
         else:
             caches = [KVCache(B, cfg.kv_heads, P + self.max_new_tokens, cfg.head_dim, dev, self.module.embed.dtype)
                       for _ in self.module.layers]
-        # prefill: the vocabulary projection of the last prompt position only
-        h = self.module(ids, caches=caches, pos0=0, audio_feats=af, image_patches=ip, return_hidden=True,
-                        **({"tp_decode": tp} if tp is not None else {}))
-        logits = self.module.lm_head(h[:, -1:].contiguous()).float()[:, -1]
+        if not self.kv8:
+            # prefill: the vocabulary projection of the last prompt position only
+            h = self.module(ids, caches=caches, pos0=0, audio_feats=af, image_patches=ip, return_hidden=True,
+                            **({"tp_decode": tp} if tp is not None else {}))
+            logits = self.module.lm_head(h[:, -1:].contiguous()).float()[:, -1]
+        history = None
+        if self.shaping is not None:
+            # prompt, then the tokens as they are drawn; the lengths in force are on the device
+            history = torch.cat([ids, ids.new_zeros(B, self.max_new_tokens)], 1)
+            said = torch.full((B,), P, dtype=torch.int32, device=dev)
+            prompt_lens = said.clone()
         out_ids, out_lp = [], []
         done = torch.zeros(B, dtype=torch.bool, device=ids.device)
         mask = []
@@ -159,9 +205,15 @@ class LLMRolloutEngine:
             self.module.rope(0, P + self.max_new_tokens, dev)  # the table covers every decode position
             step = _DecodeStep(self.module, caches, B, dev)
         for t in range(self.max_new_tokens):
+            if history is not None:
+                ok = self.allowed_tokens(history[:, P:P + t]) if self.allowed_tokens is not None else None
+                logits = process_logits(logits, history, said, prompt_lens, allowed=ok, **self.shaping)
             nxt, lp = sample_tokens(logits, self.temperature, self.top_k, self.top_p, g)
             if self.temperature <= 0:
                 lp = torch.log_softmax(logits.float(), -1).gather(-1, nxt[:, None]).squeeze(-1)
+            if history is not None:
+                history[:, P + t] = nxt
+                said += 1
             out_ids.append(nxt)
             out_lp.append(lp)
             mask.append(~done)
@@ -180,6 +232,30 @@ class LLMRolloutEngine:
             ids, lp = ids[own], lp[own]
             out_ids, mask = [t[own] for t in out_ids], [t[own] for t in mask]
         return self._pack(batch, ids, out_ids, lp, mask)
+
+    def _prefill8(self, ids, af, ip, group: int):
+        """8-bit paged caches of the batch's rows, and the logits after the prompts.  One row of every group is
+        prefilled, the others are forks of it."""
+        B, P = ids.shape
+        if group < 1 or B % group:
+            raise ValueError(f"group={group} must divide the batch of {B} rows")
+        cfg, bs, dev = self.module.cfg, self.kv_block_size or 64, ids.device
+        total = P + self.max_new_tokens
+        # per group the prompt's full pages once, then what every sample adds (the copied last page among it), and the
+        # prompt's own partly filled page while it is copied
+        pages = (B // group) * (P // bs + group * (-(-total // bs) - P // bs))
+        cache = PagedKVCache8(len(self.module.layers), pages, cfg.kv_heads, bs, cfg.head_dim, dev)
+        first = [cache.add_sequence() for _ in range(B // group)]
+        views = cache.batch(first, P).views()
+        h = self.module(ids[::group], caches=views, pos0=0, audio_feats=af[::group] if af is not None else None,
+                        image_patches=ip[::group] if ip is not None else None, return_hidden=True)
+        logits = self.module.lm_head(h[:, -1:].contiguous()).float()[:, -1].repeat_interleave(group, 0)
+        sids = first
+        if group > 1:
+            sids = [s for f, kids in zip(first, cache.fork(first, group - 1)) for s in [f, *kids]]
+        batch = cache.batch(sids, total)
+        batch.reserve(self.max_new_tokens)  # every page of the response: the block table stays as it is
+        return batch.views(), logits
 
     @staticmethod
     def _gather(t: torch.Tensor, tp) -> torch.Tensor:
