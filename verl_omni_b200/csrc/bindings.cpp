@@ -123,6 +123,7 @@ void paged8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Te
 torch::Tensor paged8_attend(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor ks, torch::Tensor vs,
                             torch::Tensor table, torch::Tensor lens, c10::optional<torch::Tensor> q_lens, double scale,
                             int64_t len_add);
+int64_t paged8_error(bool reset);
 void copy_pages(std::vector<torch::Tensor> pools, torch::Tensor src, torch::Tensor dst);
 torch::Tensor process_logits(torch::Tensor x, c10::optional<torch::Tensor> g, c10::optional<torch::Tensor> history,
                              c10::optional<torch::Tensor> lens, c10::optional<torch::Tensor> prompt_lens,
@@ -222,6 +223,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("block_table") = py::none());
   m.def("paged8_append", &vo::paged8_append, "bf16 rows into the pages of an e4m3 KV cache (power-of-two page scales)");
   m.def("paged8_attend", &vo::paged8_attend, "grouped-query attention over an e4m3 paged KV cache");
+  m.def("paged8_error", &vo::paged8_error, "first error code of a bounded wait in the 8-bit attention kernels");
   m.def("copy_pages", &vo::copy_pages, "page copies inside pools [layers, pages, ...], one launch");
   m.def("process_logits", &vo::process_logits, "penalties, bias and bitmask on logits, or their gradient");
   m.def("fmha_fwd_peer", &vo::fmha_fwd_peer, "Ulysses attention writing each output row to its owner rank",

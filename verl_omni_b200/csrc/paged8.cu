@@ -8,6 +8,7 @@
 
 #include "common.cuh"
 #include "paged8.cuh"
+#include "paged8_tc.h"
 
 namespace vo {
 namespace {
@@ -319,6 +320,11 @@ void copy_pages(std::vector<torch::Tensor> pools, torch::Tensor src, torch::Tens
   count_launch();
 }
 
+int64_t paged8_error(bool reset) {
+  const int few = paged8_decode_error(reset), many = paged8_chunk_error(reset);
+  return few ? few : many;
+}
+
 // q [B, Hq, S, hd] bf16 -> [B, S, Hq, hd]: query token i of sequence b stands at position
 // lens[b] + len_add - q_lens[b] + i and attends to the cached rows up to its own; rows past q_lens[b] and
 // rows without a key are zero.
@@ -347,6 +353,18 @@ torch::Tensor paged8_attend(torch::Tensor q, torch::Tensor kp, torch::Tensor vp,
                    vs.data_ptr<float>(), table.data_ptr<int>(), lens.data_ptr<int>(), ql,
                    reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), (int)table.size(1), (int)kp.size(0), (int)kp.size(2), (int)B,
                    (int)Hq, (int)Hk, (int)(Hq / Hk), (int)S, (int)hd, (int)len_add, (float)(scale * 1.4426950408889634)};
+  // Few rows: bound by the cache's bytes, the kernel with keys as the products' M.  Many: bound by arithmetic, rows as M.
+  // Head widths and page sizes outside both: the CUDA-core kernel.
+  const bool few = paged8_decode_ok(a);
+  if (few || paged8_chunk_ok(a)) {
+    const int sms = num_sms();
+    auto ws = torch::empty({few ? paged8_decode_workspace(a, sms) : paged8_chunk_workspace(a, sms)}, q.options().dtype(torch::kUInt8));
+    int launches = 0;
+    const int rc = (few ? paged8_decode_launch : paged8_chunk_launch)(a, ws.data_ptr(), sms, stream(), &launches);
+    TORCH_CHECK(rc == 0, "8-bit attention launch failed: ", std::to_string(rc));
+    count_launch(launches);
+    return out;
+  }
   attend_any_kernel<<<(unsigned)(B * S * Hq), 128, 0, stream()>>>(a);
   VO_CUDA_OK(cudaGetLastError());
   count_launch();

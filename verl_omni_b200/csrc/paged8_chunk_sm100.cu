@@ -1,0 +1,767 @@
+// Attention over the 8-bit paged KV cache for many query rows (chunks of a prompt, verification of several tokens, wide
+// head groups), on tcgen05.
+//
+// Here the bound is arithmetic: the exponentials and the two products of rows x keys.  Query rows (token, head of the KV
+// group) are the M of both products, 256 rows a CTA in two tiles of 128; keys and values become f16 once per 256 rows:
+// every e4m3 number is an f16 number, and the page scales, powers of two, enter as code * scale / (largest scale of the
+// CTA's key range) (exact down to 2^-24 of it).  Probabilities are f16 too (11 bits), kept in tensor memory over the scores
+// they come from; queries are brought to [2^7, 2^9) by a power of two per row, exact for bf16.  Running maximum with a
+// lazy rescale of the output (only when it grows by more than 2^8), fp32 sums.
+// Work: as in the kernel for few rows, the 128-key tiles of all (sequence, KV head, 256 rows) items form one line split
+// evenly over one CTA per SM; causal items are as long as their last row's reach; cut items are merged in key order.
+// Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-10: pages -> f16 tiles in shared memory
+// (global loads one tile ahead in registers); 11: tensor-memory allocation, MMA issue.
+#include "dcheck.cuh"
+#include "paged8.cuh"
+#include "paged8_tc.h"
+#include "tc8.cuh"
+
+namespace vo {
+namespace p8chk {
+
+using namespace tc8;
+using p8::AttendArgs;
+
+constexpr int TK = 128, TR = 128, ROWS = 2 * TR;
+constexpr int NTHREADS = 384;         // 12 warps: three per scheduler, 168 registers a thread
+constexpr int NLOAD = 96;             // threads that load and convert
+constexpr int KST = 2, VST = 2;       // K and V tiles in shared memory
+constexpr int kSegs = 4;              // buffers of per-item values between the loaders and the softmax
+constexpr float kLazy = 8.f;          // log2 growth of the maximum that is left in the probabilities
+
+__device__ int g_error = 0;
+
+template <int HD>
+struct Cfg {
+  static constexpr int TILE = TK * HD * 2;  // f16 K, V or Q tile: HD / 64 groups of 64 columns, 128 rows of 128 bytes
+  static constexpr int K_OFF = 2 * TILE;
+  static constexpr int V_OFF = K_OFF + KST * TILE;
+  static constexpr int NAN_OFF = V_OFF + VST * TILE;  // [kSegs][HD] first key with a NaN value per column
+  static constexpr int REF_OFF = NAN_OFF + kSegs * HD * 4;  // [kSegs][2] largest scales, then 2 x 4 partial maxima
+  static constexpr int BAR_OFF = REF_OFF + kSegs * 8 + 32;
+  static constexpr int NBARS = 2 * KST + 2 * VST + 8 + 2 * kSegs;
+  static constexpr int START_OFF = BAR_OFF + NBARS * 8;  // tmem slot, abort flag, start item, scan sums
+  static constexpr int BYTES = START_OFF + 24 + 8 * 12 + 1024;
+};
+
+struct Meta {
+  long long g0, g1, begin, end;  // the CTA's tiles, the tiles of the item that holds g0
+  int b, kh, rt, used;           // used: CTAs with work (entry 0)
+};
+
+struct Params {
+  AttendArgs a;
+  int RT;          // row tiles (256) of a (sequence, KV head)
+  float* part_o;   // [G][2][ROWS][HD]
+  float* part_ml;  // [G][2][ROWS][2]
+  Meta* meta;
+};
+
+// tiles of row tile rt of sequence b: up to the last key that its last query token sees (one masked tile where none is)
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, int len, int nq, int rt) {
+  const int last = min((int)(((int64_t)rt * ROWS + ROWS - 1) / a.rep), nq - 1);
+  if ((int64_t)rt * ROWS >= (int64_t)nq * a.rep) return 1;
+  const int lim = len - nq + last + 1;
+  return lim > 0 ? (lim - 1) / TK + 1 : 1;
+}
+
+struct Walk {
+  int b, kh, rt, tile, nt, len, nq;
+};
+__device__ __forceinline__ void enter_seq(Walk& w, const AttendArgs& a) {
+  const bool in = w.b < a.B;
+  w.len = in ? p8::seq_len(a, w.b) : 0;
+  w.nq = in ? p8::seq_q(a, w.b) : 0;
+}
+__device__ __forceinline__ void next_item(Walk& w, const Params& p) {
+  w.tile = 0;
+  if (++w.rt == p.RT) {
+    w.rt = 0;
+    if (++w.kh == p.a.Hk) {
+      w.kh = 0;
+      ++w.b;
+      enter_seq(w, p.a);
+    }
+  }
+  w.nt = tiles_of(p.a, w.len, w.nq, w.rt);
+}
+__device__ __forceinline__ int row_lim(const AttendArgs& a, const Walk& w, int64_t row) {
+  const int s = (int)(row / a.rep);
+  return s < w.nq ? max(0, w.len - w.nq + s + 1) : 0;
+}
+
+__device__ __forceinline__ void loader_sync() { asm volatile("bar.sync 1, 96;" ::: "memory"); }
+__device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// kind::f16 instruction descriptor with f16 operands, fp32 accumulation
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn, int b_mn) { return idesc(M, N, a_mn, b_mn); }
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+// two fp32 lanes of one instruction: r = a s + c, s += a
+__device__ __forceinline__ void ffma2(float a0, float a1, float s, float c, float& r0, float& r1) {
+  asm("{\n\t.reg .b64 x, y, z, r;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+      "fma.rn.f32x2 r, x, y, z;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "=f"(r0), "=f"(r1)
+      : "f"(a0), "f"(a1), "f"(s), "f"(c));
+}
+__device__ __forceinline__ void fadd2(float& s0, float& s1, float a0, float a1) {
+  asm("{\n\t.reg .b64 x, y, r;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "add.rn.f32x2 r, x, y;\n\tmov.b64 {%0, %1}, r;\n\t}"
+      : "+f"(s0), "+f"(s1)
+      : "f"(a0), "f"(a1));
+}
+
+template <int HD>
+__global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_constant__ Params p) {
+  using C = Cfg<HD>;
+  constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
+  uint64_t* k_full = bars;              // [KST] f16 K tile written (NLOAD)
+  uint64_t* k_empty = k_full + KST;     // [KST] its products done (commit)
+  uint64_t* v_full = k_empty + KST;     // [VST]
+  uint64_t* v_empty = v_full + VST;     // [VST]
+  uint64_t* s_full = v_empty + VST;     // [2] scores of a row tile (commit)
+  uint64_t* p_full = s_full + 2;        // [2] probabilities written (4 warps)
+  uint64_t* o_final = p_full + 2;       // [2] last product of an item done (commit)
+  uint64_t* q_full = o_final + 2;       // [2] queries written (128)
+  uint64_t* ref_full = q_full + 2;      // [kSegs] largest scales of an item known (NLOAD)
+  uint64_t* nan_full = ref_full + kSegs;  // [kSegs] all its tiles loaded (NLOAD)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::START_OFF);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* start = reinterpret_cast<int*>(tmem_slot + 2);                      // b, kh, rt, tile
+  long long* sums = reinterpret_cast<long long*>(sm + C::START_OFF + 24);  // [12]
+  int* nan_at = reinterpret_cast<int*>(sm + C::NAN_OFF);
+  float* refs = reinterpret_cast<float*>(sm + C::REF_OFF);
+  const AttendArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int64_t R = (int64_t)a.S * a.rep;
+
+  // ---- this CTA's share of the line of tiles
+  auto seq_tiles = [&](int b) {
+    const int len = p8::seq_len(a, b), nq = p8::seq_q(a, b);
+    long long n = 0;
+    for (int rt = 0; rt < p.RT; ++rt) n += tiles_of(a, len, nq, rt);
+    return n;
+  };
+  long long mine = 0;
+  const int per = (a.B + NTHREADS - 1) / NTHREADS;
+  for (int b = tid * per; b < min(a.B, (tid + 1) * per); ++b) mine += seq_tiles(b);
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  if (lane == 31) sums[warp] = upto;
+  if (tid == 0) {
+    for (int i = 0; i < KST; ++i) mbar_init(&k_full[i], NLOAD), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < VST; ++i) mbar_init(&v_full[i], NLOAD), mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_final[i], 1), mbar_init(&q_full[i], 128);
+    for (int i = 0; i < kSegs; ++i) mbar_init(&ref_full[i], NLOAD), mbar_init(&nan_full[i], NLOAD);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 11) tmem_alloc(tmem_slot, TMEM_COLS);
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < NTHREADS / 32; ++i) {
+    if (i < warp) before += sums[i];
+    total += sums[i];
+  }
+  total *= a.Hk;
+  const int used = (int)min((long long)gridDim.x, total);  // CTAs with work: one tile each at least
+  if (blockIdx.x == 0 && tid == 0) p.meta[0].used = used;
+  const bool idle = (int)blockIdx.x >= used;
+  const long long g0 = idle ? total : total * blockIdx.x / used, g1 = idle ? total : total * (blockIdx.x + 1) / used;
+  long long lo = (before + upto - mine) * a.Hk;
+  if (g0 >= lo && g0 < lo + mine * a.Hk) {
+    for (int b = tid * per;; ++b) {
+      const long long n = seq_tiles(b);
+      if (g0 < lo + n * a.Hk) {
+        const int kh = (int)((g0 - lo) / n), len = p8::seq_len(a, b), nq = p8::seq_q(a, b);
+        lo += n * kh;
+        int rt = 0, nt = tiles_of(a, len, nq, 0);
+        while (g0 >= lo + nt) {
+          lo += nt;
+          nt = tiles_of(a, len, nq, ++rt);
+        }
+        start[0] = b;
+        start[1] = kh;
+        start[2] = rt;
+        start[3] = (int)(g0 - lo);
+        Meta& me = p.meta[blockIdx.x];
+        me.g0 = g0;
+        me.g1 = g1;
+        me.begin = lo;
+        me.end = lo + nt;
+        me.b = b;
+        me.kh = kh;
+        me.rt = rt;
+        break;
+      }
+      lo += n * a.Hk;
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int ntot = (int)(g1 - g0);
+  Walk w;  // a CTA without tiles walks nothing
+  w.b = idle ? a.B : start[0];
+  w.kh = start[1];
+  w.rt = start[2];
+  w.tile = start[3];
+  enter_seq(w, a);
+  w.nt = tiles_of(a, w.len, w.nq, w.rt);
+
+  if (warp >= 8 && warp < 11) {
+    // ------------------------------------------------------------------ pages -> f16 tiles
+    constexpr int NC = HD / 16;                       // 16-byte pieces of a row
+    constexpr int RP = NLOAD / NC;                    // rows of a pass
+    constexpr int NI = (TK + RP - 1) / RP;            // passes: row i * RP + lt / NC, the last one partly empty
+    const int lt = tid - 256, lw = lt >> 5;
+    const int r_in = lt / NC, c = lt % NC;
+    // lane l < 16 holds the page of the tile's rows [8 l, 8 l + 8)
+    auto page_of = [&](const Walk& x) {
+      const int t = x.tile * TK + (lane & 15) * 8;
+      return t < x.len ? __ldg(a.table + (int64_t)x.b * a.width + t / a.block) : -1;
+    };
+    auto load = [&](const uint8_t* pool, const Walk& x, int pages, uint4 (&d)[NI]) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = i * RP + r_in, t = x.tile * TK + r;
+        const int id = __shfl_sync(0xffffffffu, pages, (r >> 3) & 15);
+        const bool ok = r < TK && t < x.len && id >= 0 && id < a.pages;
+        d[i] = make_uint4(0, 0, 0, 0);
+        if (ok) d[i] = __ldg(reinterpret_cast<const uint4*>(pool + (((int64_t)id * a.Hk + x.kh) * a.block + t % a.block) * HD + c * 16));
+      }
+    };
+    // code * scale / ref in f16, 64-column groups of swizzled 128-byte rows; the two halves of a piece are written in
+    // the other order in the odd groups, so that a row's eight lanes hit different banks
+    auto store = [&](uint8_t* dst, const uint4 (&d)[NI], float scale, float inv_ref) {
+      const float mine_f = scale * inv_ref;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = i * RP + r_in;
+        const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, mine_f, (r >> 3) & 15));
+        if (r >= TK) break;
+        const uint32_t u[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+        uint32_t h[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(j & 1 ? u[j >> 1] >> 16 : u[j >> 1] & 0xffff), __NV_E4M3);
+          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f);
+          h[j] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+        const int grp = c >> 2, i0 = (c & 3) * 2;
+        uint8_t* base = dst + grp * (TK * 128);
+        const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+        const bool odd = grp & 1;
+        *reinterpret_cast<uint4*>(base + swz<128>(r, odd ? i0 + 1 : i0)) = odd ? h1 : h0;
+        *reinterpret_cast<uint4*>(base + swz<128>(r, odd ? i0 : i0 + 1)) = odd ? h0 : h1;
+      }
+      fence_async_smem();
+    };
+    auto scale_of_page = [&](const float* sc, const Walk& x, int id) {
+      return id >= 0 && id < a.pages ? __ldg(sc + (int64_t)id * a.Hk + x.kh) : 0.f;
+    };
+    int seg = 0, i = 0, left = 0;
+    float kinv = 1.f, vinv = 1.f;
+    int common = 0, buf = 0;
+    int pg = ntot > 0 ? page_of(w) : -1;
+    uint4 kd[NI], vd[NI];
+    if (ntot > 0) load(a.kp, w, pg, kd);
+    for (; i < ntot; ++i) {
+      const float ksc = scale_of_page(a.ks, w, pg), vsc = scale_of_page(a.vs, w, pg);
+      load(a.vp, w, pg, vd);
+      if (left == 0) {
+        // largest scales over this item's part: the f16 numbers are relative to them
+        left = min(w.nt - w.tile, ntot - i);
+        buf = seg % kSegs;
+        const int p0 = w.tile * TK / a.block, p1 = (min(w.len, (w.tile + left) * TK) + a.block - 1) / a.block;
+        float km = 0.f, vm = 0.f;
+        for (int x = p0 + lt; x < p1; x += NLOAD) {
+          const int id = __ldg(a.table + (int64_t)w.b * a.width + x);
+          km = fmaxf(km, scale_of_page(a.ks, w, id));
+          vm = fmaxf(vm, scale_of_page(a.vs, w, id));
+        }
+        km = warp_fmax(km);
+        vm = warp_fmax(vm);
+        float* pm = refs + 2 * kSegs;
+        loader_sync();  // the maxima of the item before have been read
+        if (lane == 0) pm[lw] = km, pm[4 + lw] = vm;
+        loader_sync();
+        km = fmaxf(fmaxf(pm[0], pm[1]), pm[2]);
+        vm = fmaxf(fmaxf(pm[4], pm[5]), pm[6]);
+        km = km > 0.f ? km : 1.f;
+        vm = vm > 0.f ? vm : 1.f;
+        kinv = inv_pow2(km);
+        vinv = inv_pow2(vm);
+        common = max(1, w.len - w.nq + (int)((int64_t)w.rt * ROWS / a.rep) + 1);  // keys below: seen by every row that sees any
+        // buffers seg % kSegs were last read three items ago: this wait (two tiles back) is past that
+        mbar_wait(&k_empty[i % KST], ((i / KST) & 1) ^ 1, abort_flag, &g_error, 21);
+        for (int x = lt; x < HD; x += NLOAD) nan_at[buf * HD + x] = 0x7fffffff;
+        if (lt == 0) refs[buf * 2] = km, refs[buf * 2 + 1] = vm;
+        loader_sync();
+        mbar_arrive(&ref_full[buf]);
+        ++seg;
+      }
+      const Walk cur = w;
+      if (--left == 0) next_item(w, p);
+      else ++w.tile;
+      const int pg_next = i + 1 < ntot ? page_of(w) : -1;
+      mbar_wait(&k_empty[i % KST], ((i / KST) & 1) ^ 1, abort_flag, &g_error, 22);
+      store(sm + C::K_OFF + (i % KST) * C::TILE, kd, ksc, kinv);
+      mbar_arrive(&k_full[i % KST]);
+      if (i + 1 < ntot) load(a.kp, w, pg_next, kd);
+      if ((cur.tile + 1) * TK > common) {
+        // some row sees only part of this tile: a NaN value must not reach it through 0 * NaN
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+          uint32_t* u = reinterpret_cast<uint32_t*>(&vd[j]);
+          const int t = cur.tile * TK + j * RP + r_in;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if ((((u[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0) continue;
+            for (int by = 0; by < 4; ++by)
+              if (((u[q] >> (8 * by)) & 0x7f) == 0x7f) {
+                atomicMin(&nan_at[buf * HD + c * 16 + q * 4 + by], t);
+                u[q] &= ~(0xffu << (8 * by));
+              }
+          }
+        }
+      }
+      mbar_wait(&v_empty[i % VST], ((i / VST) & 1) ^ 1, abort_flag, &g_error, 23);
+      store(sm + C::V_OFF + (i % VST) * C::TILE, vd, vsc, vinv);
+      mbar_arrive(&v_full[i % VST]);
+      if (left == 0) mbar_arrive(&nan_full[buf]);
+      pg = pg_next;
+    }
+  } else if (warp == 11) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc_f16(128, 128, 0, 0), id_o = idesc_f16(128, HD, 0, 1);
+      const uint32_t base = smem_u32(sm);
+      uint64_t* last_bar = nullptr;
+      uint32_t last_par = 0;
+      auto track = [&](uint64_t* b, uint32_t par) {
+        commit(b);
+        last_bar = b;
+        last_par = par;
+      };
+      int ns[2] = {0, 0}, nq[2] = {0, 0};  // score tiles and items issued per row tile
+      auto issue_s = [&](int t, int i) {
+        const uint32_t qa = base + t * C::TILE, ka = base + C::K_OFF + (i % KST) * C::TILE;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (TK * 128) + (kk & 3) * 32;
+          mma_f16_ss(tmem + S_COL + t * 128, desc<128>(qa + off, 16, 1024), desc<128>(ka + off, 16, 1024), id_s, kk > 0);
+        }
+        track(&s_full[t], ns[t] & 1);
+        ++ns[t];
+      };
+      auto issue_pv = [&](int t, int i, bool first) {
+        const uint32_t va = base + C::V_OFF + (i % VST) * C::TILE;
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk)
+          mma_f16_ts(tmem + O_COL + t * HD, tmem + S_COL + t * 128 + kk * 8, desc<128>(va + kk * 2048, TK * 128, 1024), id_o,
+                     !first || kk > 0);
+      };
+      bool ok = true;
+      int i = 0;
+      while (ok && i < ntot) {
+        const int n = min(w.nt - w.tile, ntot - i);
+        const bool two = (int64_t)w.rt * ROWS + TR < R;
+        ok = mbar_wait(&q_full[0], nq[0] & 1, abort_flag, &g_error, 31);
+        if (ok && two) ok = mbar_wait(&q_full[1], nq[1] & 1, abort_flag, &g_error, 32);
+        ok = ok && mbar_wait(&k_full[i % KST], (i / KST) & 1, abort_flag, &g_error, 33);
+        if (!ok) break;
+        fence_after();
+        issue_s(0, i);
+        if (two) issue_s(1, i);
+        track(&k_empty[i % KST], (i / KST) & 1);
+        for (int j = 0; ok && j < n; ++j, ++i) {
+          const bool more = j + 1 < n;
+          ok = mbar_wait(&v_full[i % VST], (i / VST) & 1, abort_flag, &g_error, 34) &&
+               mbar_wait(&p_full[0], (ns[0] - 1) & 1, abort_flag, &g_error, 35);
+          if (!ok) break;
+          fence_after();
+          issue_pv(0, i, j == 0);
+          if (!two) track(&v_empty[i % VST], (i / VST) & 1);
+          if (more) {
+            ok = mbar_wait(&k_full[(i + 1) % KST], ((i + 1) / KST) & 1, abort_flag, &g_error, 36);
+            if (!ok) break;
+            fence_after();
+            issue_s(0, i + 1);
+            if (!two) track(&k_empty[(i + 1) % KST], ((i + 1) / KST) & 1);
+          } else {
+            track(&o_final[0], nq[0] & 1);
+          }
+          if (two) {
+            // (ns[1] - 1): the score tile whose probabilities these are
+            ok = mbar_wait(&p_full[1], (ns[1] - 1) & 1, abort_flag, &g_error, 37);
+            if (!ok) break;
+            fence_after();
+            issue_pv(1, i, j == 0);
+            track(&v_empty[i % VST], (i / VST) & 1);
+            if (more) {
+              issue_s(1, i + 1);
+              track(&k_empty[(i + 1) % KST], ((i + 1) / KST) & 1);
+            } else {
+              track(&o_final[1], nq[1] & 1);
+            }
+          }
+        }
+        ++nq[0];
+        if (two) ++nq[1];
+        next_item(w, p);
+      }
+      if (last_bar) mbar_drain(last_bar, last_par);
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ softmax and output of one row tile
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t S_t = tmem + S_COL + t * 128 + lane_off, O_t = tmem + O_COL + t * HD + lane_off;
+    const float sgn = a.scale_log2 < 0.f ? -1.f : 1.f;
+    int it = 0, seg = 0, ns = 0, nitem = 0;
+    while (it < ntot) {
+      const int n = min(w.nt - w.tile, ntot - it), buf = seg % kSegs;
+      const Walk cur = w;
+      const int64_t rr = (int64_t)w.rt * ROWS + t * TR + row;  // row among the (token, head) rows of the KV head
+      const bool active = (int64_t)w.rt * ROWS + t * TR < R;
+      it += n;
+      ++seg;
+      next_item(w, p);
+      if (!active) continue;  // the second row tile holds no rows: nothing is issued for it
+      const int lim_row = rr < R ? row_lim(a, cur, rr) : 0;
+      float up;
+      {
+        // queries of this row in f16, times 2^-e
+        const bool has = rr < R;
+        const __nv_bfloat16* q = a.q + cur.b * a.qsb + (int64_t)(cur.kh * a.rep + (has ? (int)(rr % a.rep) : 0)) * a.qsh +
+                                 (has ? rr / a.rep : 0) * a.qss;
+        float m = 0.f;
+        bool finite = true;
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 u = has ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
+          const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float f0 = fabsf(__uint_as_float(x[k] << 16)), f1 = fabsf(__uint_as_float(x[k] & 0xffff0000u));
+            m = fmaxf(m, fmaxf(f0, f1));
+            finite = finite && f0 <= 3.4028234e38f && f1 <= 3.4028234e38f;
+          }
+        }
+        up = !finite || m == 0.f ? 1.f : p8::scale_of(m);
+        const float inv = sgn * inv_pow2(up);
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 u = has && finite ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
+          const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(x[k] << 16) * inv, __uint_as_float(x[k] & 0xffff0000u) * inv);
+          *reinterpret_cast<uint4*>(sm + t * C::TILE + (c >> 3) * (TK * 128) + swz<128>(row, c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        if (!finite) up = __int_as_float(0x7fffffff);  // an infinity or NaN in the query: its scores are NaN
+        fence_async_smem();
+        mbar_arrive(&q_full[t]);
+      }
+      mbar_wait(&ref_full[buf], ((seg - 1) / kSegs) & 1, abort_flag, &g_error, 41);
+      const float sl2 = sgn * a.scale_log2 * up * refs[buf * 2], vref = refs[buf * 2 + 1];
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j, ++ns) {
+        const int t0 = (cur.tile + j) * TK;
+        const int lim = max(0, min(TK, lim_row - t0));  // this row sees keys [t0, t0 + lim) of the tile
+        mbar_wait(&s_full[t], ns & 1, abort_flag, &g_error, 42);
+        __syncwarp();
+        fence_after();
+        uint32_t x[32], y[32], c0[32], c1[32];
+        float mx = -INFINITY;
+        ld32_nowait(S_t + 64, x);
+        ld32_nowait(S_t + 96, y);
+        wait_ld();
+        if (lim == TK) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (64 + i < lim) mx = fmaxf(mx, __uint_as_float(x[i]));
+            if (96 + i < lim) mx = fmaxf(mx, __uint_as_float(y[i]));
+          }
+        }
+        ld32_nowait(S_t, c0);
+        ld32_nowait(S_t + 32, c1);
+        wait_ld();
+        if (lim == TK) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(c0[i]), __uint_as_float(c1[i])));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i < lim) mx = fmaxf(mx, __uint_as_float(c0[i]));
+            if (32 + i < lim) mx = fmaxf(mx, __uint_as_float(c1[i]));
+          }
+        }
+        const float m_blk = mx * sl2;
+        float alpha = 1.f;
+        const bool move = m_blk > m + kLazy || (m == -INFINITY && m_blk > -INFINITY);
+        if (move) {
+          alpha = m == -INFINITY ? 0.f : ex2(m - m_blk);
+          m = m_blk;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+          // O_t is quiescent: the product before these scores is complete, the next one waits for this warp
+#pragma unroll
+          for (int c = 0; c < HD / 32; ++c) {
+            uint32_t o[32];
+            ld32_nowait(O_t + c * 32, o);
+            wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            st32(O_t + c * 32, o);
+          }
+        }
+        const float nmb = m == -INFINITY ? 0.f : -m;
+        float rs = 0.f, rs0 = 0.f, rs1 = 0.f;
+        auto emit = [&](const uint32_t(&v)[32], int c) {  // probabilities of 32 keys, f16 pairs over the scores' columns
+          uint32_t h[16];
+          if (lim == TK) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float x0, x1;
+              ffma2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]), sl2, nmb, x0, x1);
+              const float e0 = ex2(x0), e1 = ex2(x1);
+              fadd2(rs0, rs1, e0, e1);
+              h[i] = pack_f16(e0, e1);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k = c * 32 + 2 * i;
+              const float e0 = k < lim ? ex2(fmaf(__uint_as_float(v[2 * i]), sl2, nmb)) : 0.f;
+              const float e1 = k + 1 < lim ? ex2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, nmb)) : 0.f;
+              rs += e0 + e1;
+              h[i] = pack_f16(e0, e1);
+            }
+          }
+          st16(S_t + c * 16, h);
+        };
+        ld32_nowait(S_t + 64, x);
+        emit(c0, 0);
+        emit(c1, 1);  // columns [16, 32): chunk 1's own scores start at 32
+        wait_ld();
+        ld32_nowait(S_t + 96, y);
+        emit(x, 2);
+        wait_ld();
+        emit(y, 3);
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        l = l * alpha + (rs + (rs0 + rs1));
+      }
+      mbar_wait(&o_final[t], nitem & 1, abort_flag, &g_error, 43);
+      mbar_wait(&nan_full[buf], ((seg - 1) / kSegs) & 1, abort_flag, &g_error, 44);
+      ++nitem;
+      __syncwarp();
+      fence_after();
+      const bool from_start = cur.tile == 0, whole = from_start && n == cur.nt;
+      const float mul = whole ? (l == 0.f ? 0.f : vref / l) : vref;
+      const int64_t slot = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * ROWS + t * TR + row;
+      const int64_t orow = ((int64_t)cur.b * a.S + rr / a.rep) * a.Hq + cur.kh * a.rep + rr % a.rep;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t o[32];
+        ld32_nowait(O_t + c * 32, o);
+        wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float f = __uint_as_float(o[i]) * mul;
+          if (whole && l == 0.f) f = 0.f;  // a row without keys (a NaN among the tile's values would stay NaN)
+          if (nan_at[buf * HD + c * 32 + i] < lim_row) f = __int_as_float(0x7fffffff);
+          o[i] = __float_as_uint(f);
+        }
+        if (rr < R) {
+          if (whole) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              uint32_t h[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 b2 = __floats2bfloat162_rn(__uint_as_float(o[g * 8 + 2 * i]), __uint_as_float(o[g * 8 + 2 * i + 1]));
+                h[i] = *reinterpret_cast<const uint32_t*>(&b2);
+              }
+              *reinterpret_cast<uint4*>(a.out + orow * HD + c * 32 + g * 8) = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          } else {
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              *reinterpret_cast<uint4*>(p.part_o + slot * HD + c * 32 + g * 4) = make_uint4(o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]);
+          }
+        }
+      }
+      if (!whole && rr < R) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m, l);
+      fence_before();
+    }
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 11) {
+    __syncwarp();
+    tmem_free(tmem, TMEM_COLS);
+  }
+}
+
+// Merges the partials of items that CTA borders cut; blocks (c, 8 rows), a warp per row, in the order of the keys.
+template <int HD>
+__global__ void __launch_bounds__(256) merge8_kernel(const __grid_constant__ Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const AttendArgs& a = p.a;
+  const int c = blockIdx.x + 1, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int used = p.meta[0].used;
+  if (c >= used) return;
+  const Meta me = p.meta[c];
+  if (!(me.begin < me.g0 && me.begin >= p.meta[c - 1].g0)) return;
+  const int64_t rr = (int64_t)me.rt * ROWS + r;
+  if (rr >= (int64_t)a.S * a.rep) return;
+  constexpr int V = HD / 32;
+  float m = -INFINITY;
+  auto row_of = [&](int i) -> int64_t { return i == c - 1 ? ((int64_t)i * 2 + 1) * ROWS + r : (int64_t)i * 2 * ROWS + r; };
+  int last = c;
+  for (; last < used && p.meta[last].g0 < me.end; ++last) {
+  }
+  for (int i = c - 1; i < last; ++i) m = fmaxf(m, p.part_ml[row_of(i) * 2]);
+  float l = 0.f, o[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) o[k] = 0.f;
+  for (int i = c - 1; i < last; ++i) {
+    const int64_t x = row_of(i);
+    const float w = m == -INFINITY ? 1.f : ex2(p.part_ml[x * 2] - m);
+    l += p.part_ml[x * 2 + 1] * w;
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] += p.part_o[x * HD + lane * V + k] * w;
+  }
+  const int64_t orow = ((int64_t)me.b * a.S + rr / a.rep) * a.Hq + me.kh * a.rep + rr % a.rep;
+#pragma unroll
+  for (int k = 0; k < V; ++k) a.out[orow * HD + lane * V + k] = __float2bfloat16_rn(l == 0.f ? 0.f : o[k] / l);
+}
+
+template <int HD>
+int launch(const Params& p, int G, cudaStream_t stream, int* launches) {
+  static const cudaError_t set = cudaFuncSetAttribute(chunk8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES);
+  if (set != cudaSuccess) return (int)set;
+  chunk8_kernel<HD><<<G, NTHREADS, Cfg<HD>::BYTES, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  ++*launches;
+  if (G == 1) return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(G - 1, ROWS / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, merge8_kernel<HD>, p);
+  if (e != cudaSuccess) return (int)e;
+  ++*launches;
+  return 0;
+}
+
+int64_t row_tiles(const AttendArgs& a) { return ((int64_t)a.S * a.rep + ROWS - 1) / ROWS; }
+int ctas(const AttendArgs& a, int sms) {
+  const int64_t reach = ((int64_t)a.width * a.block + TK - 1) / TK;
+  const int64_t most = (int64_t)a.B * a.Hk * row_tiles(a) * (reach < 1 ? 1 : reach);
+  return (int)(most < sms ? most : sms);
+}
+
+}  // namespace p8chk
+
+bool paged8_chunk_ok(const p8::AttendArgs& a) {
+  return (a.hd == 64 || a.hd == 128) && paged8_pages_ok(a) && (int64_t)a.S * a.rep < (1ll << 30);
+}
+
+int64_t paged8_chunk_workspace(const p8::AttendArgs& a, int sms) {
+  const int64_t G = p8chk::ctas(a, sms);
+  return G * 2 * p8chk::ROWS * (a.hd + 2) * 4 + G * (int64_t)sizeof(p8chk::Meta);
+}
+
+int paged8_chunk_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaStream_t stream, int* launches) {
+  using namespace p8chk;
+  const int G = ctas(a, sms);
+  Params p;
+  p.a = a;
+  p.RT = (int)row_tiles(a);
+  p.part_o = static_cast<float*>(workspace);  // 16-byte rows first
+  p.part_ml = p.part_o + (int64_t)G * 2 * ROWS * a.hd;
+  p.meta = reinterpret_cast<Meta*>(p.part_ml + (int64_t)G * 2 * ROWS * 2);
+  return a.hd == 128 ? launch<128>(p, G, stream, launches) : launch<64>(p, G, stream, launches);
+}
+
+int paged8_chunk_error(bool reset) {
+  int h = 0;
+  if (cudaMemcpyFromSymbol(&h, p8chk::g_error, sizeof(int)) != cudaSuccess) return -1;
+  if (reset && h) {
+    const int z = 0;
+    cudaMemcpyToSymbol(p8chk::g_error, &z, sizeof(int));
+  }
+  return h;
+}
+
+}  // namespace vo

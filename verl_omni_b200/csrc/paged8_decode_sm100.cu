@@ -1,0 +1,645 @@
+// Attention over the 8-bit paged KV cache for few query rows (query tokens x heads of a KV group <= 16), on tcgen05.
+//
+//   o = softmax(scale q k^T) v,  k = code * k_scale[page],  v = code * v_scale[page]  (scales: powers of two)
+//
+// The bound is the cache's bytes: 2 * head_dim bytes per row and KV head, read once for all query heads of the group.
+// The e4m3 codes go from global memory to the tensor core as they are: a 128-key tile of K and V is staged by TMA, and
+// both products take it from shared memory (S^T = K Q^T: keys as M, rows as N; O^T = V^T P^T: dims as M).  The other
+// operand keeps its precision as a sum of two e4m3 numbers: q = 2^e (q_hi + q_lo) holds every bit of a bf16 query whose
+// elements lie within 2^10 of the row's largest (below that, 2^-19 of the largest), p likewise to 8 bits; two products
+// accumulate into the same fp32 columns.  Page scales stay outside: k_scale multiplies the thread's (key's) scores, the
+// v scales of a tile enter as p * v_scale / max(v_scale) and the maximum as a factor of the folded output.
+//
+// Work: the tiles of all (sequence, KV head) items form one line that the CTAs split evenly (two CTAs per SM, as many as
+// there are tiles at most), so ragged lengths balance and a long single sequence fills the GPU.  An item inside one CTA
+// is finished there; one cut by a border leaves (maximum, sum, output) partials that the combine kernel merges in
+// the order of the keys, so results do not depend on timing.
+// Warps 0-3: softmax (thread = key) and output (thread = head-dim column); 4: TMA producer, page ids read two tiles and
+// scales one tile ahead; 5: tensor-memory allocation, MMA issue (scores one tile ahead of the softmax).
+#include "dcheck.cuh"
+#include "paged8.cuh"
+#include "paged8_tc.h"
+#include "tc8.cuh"
+
+namespace vo {
+namespace p8dec {
+
+using namespace tc8;
+using p8::AttendArgs;
+
+constexpr int TK = 128;        // keys per tile
+constexpr int NB = 16;         // MMA N: query rows, zero-padded
+constexpr int NTHREADS = 192;
+constexpr int kMaxBlocksPerTile = 16;  // pages of 8 rows
+constexpr float kPOne = 256.f;         // probabilities are held times 2^8 (e4m3 reaches 448)
+
+__device__ int g_error = 0;
+
+template <int HD>
+struct Cfg {
+  static constexpr int KV = TK * HD;                    // bytes of K or V of a tile
+  static constexpr int STAGE = 2 * KV;
+  static constexpr int STAGES = HD == 128 ? 3 : 6;      // 96 KB: two CTAs per SM
+  static constexpr int Q_OFF = STAGES * STAGE;          // q_hi, q_lo: NB rows of HD bytes
+  static constexpr int P_OFF = Q_OFF + 2 * NB * HD;     // two buffers of (p_hi, p_lo): NB rows of TK bytes
+  static constexpr int SC_OFF = P_OFF + 4 * NB * TK;    // per stage: k and v scale of each page
+  static constexpr int RED_OFF = SC_OFF + STAGES * 2 * kMaxBlocksPerTile * 4;  // [2][NB + 1][4] warp maxima
+  static constexpr int QS_OFF = RED_OFF + 2 * (NB + 1) * 16;                   // [2][NB] row factors
+  static constexpr int BAR_OFF = QS_OFF + 2 * NB * 4;
+  static constexpr int NBARS = 2 * STAGES + 11;
+  static constexpr int START_OFF = BAR_OFF + NBARS * 8;  // tmem slot, abort flag, start item, scan sums
+  static constexpr int BYTES = START_OFF + 96 + 1024;
+};
+
+struct Meta {
+  long long g0, g1, begin, end;  // the CTA's tiles, the tiles of the item that holds g0
+  int item, used;                // used: CTAs with work (entry 0)
+};
+
+struct Params {
+  AttendArgs a;
+  float* part_o;   // [G][2][NR][HD]
+  float* part_ml;  // [G][2][NR][2]
+  Meta* meta;      // [G]
+};
+
+struct Walk {
+  int b, kh, tile, nt, len;
+};
+__device__ __forceinline__ int tiles_of(int len) { return len > 0 ? (len - 1) / TK + 1 : 1; }  // an empty sequence: one masked tile
+__device__ __forceinline__ void enter(Walk& w, const AttendArgs& a) {
+  w.len = w.b < a.B ? p8::seq_len(a, w.b) : 0;
+  w.nt = tiles_of(w.len);
+}
+__device__ __forceinline__ void next_item(Walk& w, const AttendArgs& a) {
+  w.tile = 0;
+  if (++w.kh == a.Hk) {
+    w.kh = 0;
+    ++w.b;
+    enter(w, a);
+  }
+}
+
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
+
+template <int HD, int NR, bool CAUSAL>
+__global__ void __launch_bounds__(NTHREADS, 2)
+    decode8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params p) {
+  using C = Cfg<HD>;
+  constexpr int STAGES = C::STAGES;
+  constexpr uint32_t TMEM_COLS = 64, S_COL = 0, O_COL = 32;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
+  uint64_t* full = bars;                 // [STAGES] tile landed (1 + tx)
+  uint64_t* kv_empty = full + STAGES;    // [STAGES] its PV products done (commit)
+  uint64_t* s_full = kv_empty + STAGES;  // [2] scores in tensor memory (commit)
+  uint64_t* s_empty = s_full + 2;        // [2] scores read (128)
+  uint64_t* p_full = s_empty + 2;        // [2] probabilities written (128)
+  uint64_t* o_full = p_full + 2;         // [2] tile output in tensor memory (commit)
+  uint64_t* o_empty = o_full + 2;        // [2] tile output read (128)
+  uint64_t* q_full = o_empty + 2;        // queries of the next item written (128)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::START_OFF);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* start = reinterpret_cast<int*>(tmem_slot + 2);                      // b, kh, tile of the first tile
+  long long* sums = reinterpret_cast<long long*>(sm + C::START_OFF + 24);  // [6] per-warp tile counts
+  float* scl = reinterpret_cast<float*>(sm + C::SC_OFF);
+  float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
+  float* qsc = reinterpret_cast<float*>(sm + C::QS_OFF);
+  const AttendArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+
+  // ---- this CTA's share [g0, g1) of the line of tiles, and the item that holds g0
+  long long mine = 0;
+  const int per = (a.B + NTHREADS - 1) / NTHREADS;
+  for (int b = tid * per; b < min(a.B, (tid + 1) * per); ++b) mine += tiles_of(p8::seq_len(a, b));
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  if (lane == 31) sums[warp] = upto;
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 128);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 128);
+    }
+    mbar_init(q_full, 128);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+  }
+  if (warp == 5) tmem_alloc(tmem_slot, TMEM_COLS);
+  if (warp < 4)  // rows past the queries and heads stay zero for the whole kernel
+    for (int u = tid; u < (C::SC_OFF - C::Q_OFF) / 16; u += 128) reinterpret_cast<uint4*>(sm + C::Q_OFF)[u] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < NTHREADS / 32; ++i) {
+    if (i < warp) before += sums[i];
+    total += sums[i];
+  }
+  total *= a.Hk;
+  const int used = (int)min((long long)gridDim.x, total);  // CTAs with work: one tile each at least
+  if (blockIdx.x == 0 && tid == 0) p.meta[0].used = used;
+  const bool idle = (int)blockIdx.x >= used;
+  const long long g0 = idle ? total : total * blockIdx.x / used, g1 = idle ? total : total * (blockIdx.x + 1) / used;
+  long long lo = (before + upto - mine) * a.Hk;
+  if (g0 >= lo && g0 < lo + mine * a.Hk) {
+    for (int b = tid * per;; ++b) {
+      const int nt = tiles_of(p8::seq_len(a, b));
+      if (g0 < lo + (long long)nt * a.Hk) {
+        const int kh = (int)((g0 - lo) / nt);
+        start[0] = b;
+        start[1] = kh;
+        start[2] = (int)((g0 - lo) % nt);
+        const long long begin = lo + (long long)kh * nt;
+        Meta& me = p.meta[blockIdx.x];
+        me.g0 = g0;
+        me.g1 = g1;
+        me.begin = begin;
+        me.end = begin + nt;
+        me.item = b * a.Hk + kh;
+        break;
+      }
+      lo += (long long)nt * a.Hk;
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int ntot = (int)(g1 - g0);
+  Walk w;  // a CTA without tiles walks nothing
+  w.b = idle ? a.B : start[0];
+  w.kh = start[1];
+  w.tile = start[2];
+  enter(w, a);
+
+  if (warp == 4) {
+    // ------------------------------------------------------------------ TMA producer
+    const int blk = min(a.block, TK), nblk = TK / blk;
+    struct Pre {
+      int id, kh, row;  // page of this lane (-2: no keys there), KV head, first row inside the page
+    };
+    auto fetch = [&](Pre& f) {
+      const int t0 = w.tile * TK, t = t0 + lane * blk;
+      f.id = lane < nblk && t < w.len ? __ldg(a.table + (int64_t)w.b * a.width + t / a.block) : -2;
+      f.kh = w.kh;
+      f.row = a.block > TK ? t0 % a.block : 0;
+      if (++w.tile == w.nt) next_item(w, a);
+    };
+    auto in_pool = [&](const Pre& f) { return f.id >= 0 && f.id < a.pages; };
+    auto scales = [&](const Pre& f) {
+      const int64_t i = (int64_t)f.id * a.Hk + f.kh;
+      return in_pool(f) ? make_float2(__ldg(a.ks + i), __ldg(a.vs + i)) : make_float2(0.f, 0.f);
+    };
+    Pre f0{-2, 0, 0}, f1{-2, 0, 0};
+    if (ntot > 0) fetch(f0);
+    if (ntot > 1) fetch(f1);
+    float2 s0 = scales(f0);
+    int st = 0, ph = 0, issued = 0;
+    for (int i = 0; i < ntot; ++i) {
+      Pre f2{-2, 0, 0};
+      if (i + 2 < ntot) fetch(f2);
+      const float2 s1 = scales(f1);
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(&kv_empty[st], ph ^ 1, abort_flag, &g_error, 1);
+      if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
+      if (lane < nblk) {
+        scl[(st * 2) * kMaxBlocksPerTile + lane] = s0.x;  // 0: no such page, its rows read as zeros
+        scl[(st * 2 + 1) * kMaxBlocksPerTile + lane] = s0.y;
+      }
+      const bool load = in_pool(f0);
+      (void)VO_DCHECK(load || f0.id == -2);  // checked builds record a page id outside the pool
+      const unsigned n = __popc(__ballot_sync(0xffffffffu, load));
+      if (lane == 0) mbar_expect_tx(&full[st], n * 2u * blk * HD);
+      __syncwarp();
+      if (load) {
+        const int row = (f0.id * a.Hk + f0.kh) * a.block + f0.row;
+        const uint32_t dst = smem_u32(sm) + st * C::STAGE + lane * blk * HD;
+        tma_load_2d(dst, &mk, &full[st], 0, row);
+        tma_load_2d(dst + C::KV, &mv, &full[st], 0, row);
+      }
+      issued = i + 1;
+      f0 = f1;
+      f1 = f2;
+      s0 = s1;
+      if (++st == STAGES) st = 0, ph ^= 1;
+    }
+    if (lane == 0 && *abort_flag)  // the copies in flight land before the CTA leaves
+      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_drain(&full[i % STAGES], (i / STAGES) & 1);
+    __syncwarp();
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t id_s = idesc(128, NB, 0, 0);  // K (K-major) x Q (K-major)
+      constexpr uint32_t id_o = idesc(128, NB, 1, 0);  // V (read MN-major) x P (K-major)
+      const uint32_t base = smem_u32(sm);
+      uint64_t* last_bar = nullptr;  // the latest commit: its completion covers every product issued
+      uint32_t last_par = 0;
+      int st_s = 0, ph_s = 0, st_o = 0, left = 0, seg = 0;
+      auto issue_s = [&](int i) {
+        if (left == 0) {  // first tile of an item: its queries
+          left = min(w.nt - w.tile, ntot - i);
+          if (!mbar_wait(q_full, seg & 1, abort_flag, &g_error, 2)) return false;
+          ++seg;
+          next_item(w, a);
+        }
+        --left;
+        const int sb = i & 1;
+        if (!mbar_wait(&full[st_s], ph_s, abort_flag, &g_error, 3) ||
+            !mbar_wait(&s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 4))
+          return false;
+        fence_after();
+        const uint32_t ka = base + st_s * C::STAGE, qa = base + C::Q_OFF;
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int kk = 0; kk < HD / 32; ++kk)
+            mma_ss(tmem + S_COL + sb * NB, desc<HD>(ka + kk * 32, 16, 8 * HD), desc<HD>(qa + part * NB * HD + kk * 32, 16, 8 * HD),
+                   id_s, part + kk > 0 ? 1u : 0u);
+        commit(&s_full[sb]);
+        last_bar = &s_full[sb];
+        last_par = (i >> 1) & 1;
+        if (++st_s == STAGES) st_s = 0, ph_s ^= 1;
+        return true;
+      };
+      auto issue_pv = [&](int i) {
+        const int sb = i & 1;
+        if (!mbar_wait(&p_full[sb], (i >> 1) & 1, abort_flag, &g_error, 5) ||
+            !mbar_wait(&o_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 6))
+          return false;
+        fence_after();
+        const uint32_t va = base + st_o * C::STAGE + C::KV, pa = base + C::P_OFF + sb * 2 * NB * TK;
+        // head_dim 64: the second half of the 128 lanes repeats the first (stride 0 between 64-dim groups), unused
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int kk = 0; kk < TK / 32; ++kk)
+            mma_ss(tmem + O_COL + sb * NB, desc<HD>(va + kk * 32 * HD, 0, 8 * HD), desc<128>(pa + part * NB * TK + kk * 32, 16, 1024),
+                   id_o, part + kk > 0 ? 1u : 0u);
+        commit(&o_full[sb]);
+        commit(&kv_empty[st_o]);
+        last_bar = &kv_empty[st_o];
+        last_par = (i / STAGES) & 1;
+        if (++st_o == STAGES) st_o = 0;
+        return true;
+      };
+      bool ok = ntot > 0 && issue_s(0);
+      for (int i = 0; i < ntot && ok; ++i) {
+        if (i + 1 < ntot) ok = issue_s(i + 1);
+        if (ok) ok = issue_pv(i);
+      }
+      if (last_bar) mbar_drain(last_bar, last_par);  // before tensor memory is released
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax and output (warps 0-3)
+    const int R = a.S * a.rep;  // query rows of an item, <= NR
+    // queries of item (b, kh): thread = 8 consecutive elements of a row; row factor 2^e * scale goes to the scores
+    auto load_q = [&](int b, int kh, int buf) {
+      constexpr int LPR = HD / 8;  // lanes per row
+#pragma unroll
+      for (int r = tid / LPR; r < NR; r += 128 / LPR) {
+        float f[8];
+        const int c = tid % LPR;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < R) {
+          const int s = r / a.rep, h = kh * a.rep + r % a.rep;
+          u = *reinterpret_cast<const uint4*>(a.q + b * a.qsb + h * a.qsh + s * a.qss + c * 8);
+        }
+        const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+        float m = 0.f;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = __uint_as_float(uw[i] << 16);
+          f[2 * i + 1] = __uint_as_float(uw[i] & 0xffff0000u);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          m = fmaxf(m, fabsf(f[i]));
+          finite = finite && fabsf(f[i]) <= 3.4028234e38f;
+        }
+        if (!finite) m = INFINITY;
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const bool bad = m == INFINITY;  // a row with an infinity or NaN: its scores are NaN
+        const float up = m == 0.f || bad ? 1.f : p8::scale_of(m), inv = inv_pow2(up);
+        float lo8[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = bad ? 0.f : f[i] * inv;
+        const uint2 hi = p8::pack_e4m3x8(f);
+        p8::unpack_e4m3x8(hi, lo8);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lo8[i] = f[i] - lo8[i];
+        uint8_t* q = sm + C::Q_OFF + swz<HD>(r, c >> 1) + (c & 1) * 8;
+        *reinterpret_cast<uint2*>(q) = hi;
+        *reinterpret_cast<uint2*>(q + NB * HD) = p8::pack_e4m3x8(lo8);
+        if (c == 0) qsc[buf * NB + r] = bad ? __int_as_float(0x7fffffff) : a.scale_log2 * up;
+      }
+      fence_async_smem();
+      mbar_arrive(q_full);
+    };
+    const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
+    const int blk = min(a.block, TK), my_blk = tid / blk;
+    int st = 0, seg = 0, it = 0;
+    if (ntot > 0) load_q(w.b, w.kh, 0);
+    while (it < ntot) {
+      const int nseg = min(w.nt - w.tile, ntot - it), nq = p8::seq_q(a, w.b);
+      const bool from_start = w.tile == 0, whole = from_start && nseg == w.nt;
+      float m[NR], lpart[NR], acc[NR], alpha[NR], qf[NR];
+      int lim[CAUSAL ? NR : 1];
+      float vfac = 0.f;
+      int nan_at = 0x7fffffff;  // first key whose value in this thread's column is NaN (tiles that a row sees partly)
+      compute_sync();           // row factors of this item are written
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        m[h] = -INFINITY;
+        lpart[h] = acc[h] = 0.f;
+        alpha[h] = 1.f;
+        qf[h] = qsc[(seg & 1) * NB + h];
+        if (CAUSAL) {
+          const int s = h / a.rep;
+          lim[h] = h < R && s < nq ? max(0, w.len - nq + s + 1) : 0;
+        }
+      }
+      if (!CAUSAL) lim[0] = nq > 0 ? w.len : 0;
+      const int common = CAUSAL ? max(1, w.len - nq + 1) : w.len;  // keys below it are seen by every row that sees any
+      auto fold = [&](int i) {  // thread = head-dim column: acc = acc * alpha_i + O_i
+        const int sb = i & 1;
+        mbar_wait(&o_full[sb], (i >> 1) & 1, abort_flag, &g_error, 7);
+        __syncwarp();
+        fence_after();
+        uint32_t r[NR];
+        ld_nowait(trow + O_COL + sb * NB, r);
+        wait_ld();
+        fence_before();
+        mbar_arrive(&o_empty[sb]);
+#pragma unroll
+        for (int h = 0; h < NR; ++h) acc[h] = fmaf(acc[h], alpha[h], __uint_as_float(r[h]) * vfac);
+      };
+      const Walk cur = w;
+      next_item(w, a);
+      for (int j = 0; j < nseg; ++j) {
+        const int i = it + j, sb = i & 1, t0 = (cur.tile + j) * TK, t = t0 + tid;
+        mbar_wait(&full[st], (i / STAGES) & 1, abort_flag, &g_error, 8);
+        mbar_wait(&s_full[sb], (i >> 1) & 1, abort_flag, &g_error, 9);
+        __syncwarp();
+        fence_after();
+        uint32_t r[NR];
+        ld_nowait(trow + S_COL + sb * NB, r);
+        const float ksc = scl[(st * 2) * kMaxBlocksPerTile + my_blk];
+        const bool there = t < cur.len;
+        const float vsc = there ? scl[(st * 2 + 1) * kMaxBlocksPerTile + my_blk] : 0.f;
+        wait_ld();
+        fence_before();
+        mbar_arrive(&s_empty[sb]);
+        float s[NR];
+        float* rd = red + sb * (NB + 1) * 4;
+#pragma unroll
+        for (int h = 0; h < NR; ++h) {
+          const bool seen = CAUSAL ? t < lim[h] : t < lim[0];
+          s[h] = !seen ? -INFINITY : ksc == 0.f ? 0.f : __uint_as_float(r[h]) * (ksc * qf[h]);
+          const float v = warp_fmax(s[h]);
+          if (lane == 0) rd[h * 4 + warp] = v;
+        }
+        {
+          const float v = warp_fmax(vsc);
+          if (lane == 0) rd[NB * 4 + warp] = v;
+        }
+        compute_sync();
+        const float4 v4 = *reinterpret_cast<const float4*>(rd + NB * 4);
+        const float vmax = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
+        const float vr = vmax > 0.f ? vsc * inv_pow2(vmax) * kPOne : 0.f;
+        float alpha_now[NR], pv[NR];
+#pragma unroll
+        for (int h = 0; h < NR; ++h) {
+          const float4 x = *reinterpret_cast<const float4*>(rd + h * 4);
+          const float mn = fmaxf(m[h], fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
+          alpha_now[h] = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
+          const float e = s[h] == -INFINITY ? 0.f : ex2(s[h] - mn);
+          lpart[h] = fmaf(lpart[h], alpha_now[h], e);
+          m[h] = mn;
+          pv[h] = e * vr;
+        }
+        uint8_t* pb = sm + C::P_OFF + sb * 2 * NB * TK;
+#pragma unroll
+        for (int h = 0; h < NR; h += 2) {
+          const uint16_t hi = p8::float2_to_e4m3x2(pv[h], pv[h + 1]);
+          const float2 back = p8::e4m3x2_to_float2(hi);
+          const uint16_t lo2 = p8::float2_to_e4m3x2(pv[h] - back.x, pv[h + 1] - back.y);
+          uint8_t* d0 = pb + swz<128>(h, tid >> 4) + (tid & 15);
+          uint8_t* d1 = pb + swz<128>(h + 1, tid >> 4) + (tid & 15);
+          d0[0] = (uint8_t)hi;
+          d1[0] = (uint8_t)(hi >> 8);
+          d0[NB * TK] = (uint8_t)lo2;
+          d1[NB * TK] = (uint8_t)(lo2 >> 8);
+        }
+        uint8_t* vt = sm + st * C::STAGE + C::KV;
+        if (!there || vsc == 0.f) {  // rows that hold nothing: zero, so that 0 * garbage stays 0
+#pragma unroll
+          for (int c = 0; c < HD / 16; ++c) reinterpret_cast<uint4*>(vt + tid * HD)[c] = make_uint4(0, 0, 0, 0);
+        }
+        if (CAUSAL && t0 + TK > common && tid < HD) {
+          // some row sees only part of this tile: a NaN value must not reach it through 0 * NaN
+          for (int k = 0; k < min(TK, cur.len - t0); ++k) {
+            uint8_t* v = vt + swz<HD>(k, tid >> 4) + (tid & 15);
+            if ((*v & 0x7f) == 0x7f) {
+              *v = 0;
+              nan_at = min(nan_at, t0 + k);
+            }
+          }
+        }
+        fence_async_smem();
+        mbar_arrive(&p_full[sb]);
+        if (j + 1 == nseg && it + nseg < ntot) load_q(w.b, w.kh, (seg & 1) ^ 1);  // scores of this item are all read
+        if (j > 0) fold(i - 1);
+#pragma unroll
+        for (int h = 0; h < NR; ++h) alpha[h] = alpha_now[h];
+        vfac = vmax * (1.f / kPOne);
+        if (++st == STAGES) st = 0;
+      }
+      fold(it + nseg - 1);
+      // sums over the keys' threads
+      compute_sync();
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        float v = lpart[h];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) red[h * 4 + warp] = v;
+      }
+      compute_sync();
+      const int64_t slot = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * NR;
+#pragma unroll
+      for (int h = 0; h < NR; ++h) {
+        if (h >= R) break;
+        const float4 x = *reinterpret_cast<const float4*>(red + h * 4);
+        const float l = (x.x + x.y) + (x.z + x.w);
+        float o = acc[h];
+        if (CAUSAL && lim[h] > nan_at) o = __int_as_float(0x7fffffff);
+        if (tid < HD) {
+          if (whole) {
+            const int64_t row = ((int64_t)cur.b * a.S + h / a.rep) * a.Hq + cur.kh * a.rep + h % a.rep;
+            a.out[row * HD + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+          } else {
+            p.part_o[(slot + h) * HD + tid] = o;
+          }
+        }
+        if (!whole && tid == h) {
+          p.part_ml[(slot + h) * 2] = m[h];
+          p.part_ml[(slot + h) * 2 + 1] = l;
+        }
+      }
+      compute_sync();  // the sums are read before the next item's maxima overwrite them
+      it += nseg;
+      ++seg;
+    }
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 5) tmem_free(tmem, TMEM_COLS);
+}
+
+// Merges the partials of an item that CTA borders cut: block (c, row) acts where border c is the first inside its item.
+// Part 0 is slot 1 of the CTA before, the others slot 0 of CTAs c, c + 1, ...; four groups of HD threads take every
+// fourth part and are summed in a fixed order.
+template <int HD, int NR>
+__global__ void __launch_bounds__(4 * HD) combine8_kernel(const AttendArgs a, const float* __restrict__ part_o,
+                                                          const float* __restrict__ part_ml, const Meta* __restrict__ meta) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ float so[4][HD], sl[4], smx[4];
+  const int c = blockIdx.x + 1, r = blockIdx.y, grp = threadIdx.x / HD, d = threadIdx.x % HD;
+  const int used = meta[0].used;
+  if (c >= used) return;
+  const Meta me = meta[c];
+  if (!(me.begin < me.g0 && me.begin >= meta[c - 1].g0)) return;
+  int last = c;  // one past the last CTA with a part
+  while (last < used && meta[last].g0 < me.end) ++last;
+  const int parts = last - c + 1;
+  auto row_of = [&](int i) -> int64_t { return i == 0 ? ((int64_t)(c - 1) * 2 + 1) * NR + r : (int64_t)(c + i - 1) * 2 * NR + r; };
+  float m = -INFINITY;
+  for (int i = grp; i < parts; i += 4) m = fmaxf(m, part_ml[row_of(i) * 2]);
+  if (d == 0) smx[grp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
+  float l = 0.f, o = 0.f;
+#pragma unroll 4
+  for (int i = grp; i < parts; i += 4) {
+    const float w = m == -INFINITY ? 1.f : ex2(part_ml[row_of(i) * 2] - m);
+    l += part_ml[row_of(i) * 2 + 1] * w;
+    o += part_o[row_of(i) * HD + d] * w;
+  }
+  so[grp][d] = o;
+  if (d == 0) sl[grp] = l;
+  __syncthreads();
+  if (grp == 0) {
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    o = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+    const int b = me.item / a.Hk, kh = me.item % a.Hk;
+    const int64_t row = ((int64_t)b * a.S + r / a.rep) * a.Hq + kh * a.rep + r % a.rep;
+    a.out[row * HD + d] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+  }
+}
+
+template <int HD, int NR, bool CAUSAL>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, cudaStream_t stream, int* launches) {
+  static const cudaError_t set =
+      cudaFuncSetAttribute(decode8_kernel<HD, NR, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES);
+  if (set != cudaSuccess) return (int)set;
+  decode8_kernel<HD, NR, CAUSAL><<<G, NTHREADS, Cfg<HD>::BYTES, stream>>>(mk, mv, p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  ++*launches;
+  if (G == 1) return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(G - 1, p.a.S * p.a.rep);
+  cfg.blockDim = dim3(4 * HD);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, combine8_kernel<HD, NR>, p.a, (const float*)p.part_o, (const float*)p.part_ml, (const Meta*)p.meta);
+  if (e != cudaSuccess) return (int)e;
+  ++*launches;
+  return 0;
+}
+
+template <int HD>
+int pick(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, int NR, cudaStream_t stream, int* launches) {
+  const bool causal = p.a.S > 1;
+#define VO_D8(N) \
+  if (NR == N) return causal ? launch<HD, N, true>(mk, mv, p, G, stream, launches) : launch<HD, N, false>(mk, mv, p, G, stream, launches);
+  VO_D8(4) VO_D8(8) VO_D8(16)
+#undef VO_D8
+  return -1;
+}
+
+// row slots of a CTA: the query rows rounded up to 4, 8 or 16
+int rows_of(int64_t r) { return r <= 4 ? 4 : r <= 8 ? 8 : 16; }
+
+// CTAs: two per SM, one tile each at least (by the table's reach: the lengths are on the device)
+int ctas(const AttendArgs& a, int sms) {
+  const int64_t reach = ((int64_t)a.width * a.block + TK - 1) / TK;
+  const int64_t most = (int64_t)a.B * a.Hk * (reach < 1 ? 1 : reach);
+  return (int)(most < 2 * sms ? most : 2 * sms);
+}
+
+}  // namespace p8dec
+
+bool paged8_decode_ok(const p8::AttendArgs& a) {
+  if (a.hd != 64 && a.hd != 128) return false;
+  if ((int64_t)a.S * a.rep > p8dec::NB) return false;
+  return paged8_pages_ok(a);
+}
+
+int64_t paged8_decode_workspace(const p8::AttendArgs& a, int sms) {
+  const int64_t G = p8dec::ctas(a, sms), NR = p8dec::rows_of((int64_t)a.S * a.rep);
+  return G * 2 * NR * (a.hd + 2) * 4 + G * (int64_t)sizeof(p8dec::Meta);
+}
+
+int paged8_decode_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaStream_t stream, int* launches) {
+  using namespace p8dec;
+  CUtensorMap mk, mv;
+  const int64_t rows = (int64_t)a.pages * a.Hk * a.block;
+  const int box = a.block < TK ? a.block : TK;
+  int e = map_rows(&mk, a.kp, rows, a.hd, box);
+  if (e) return e;
+  e = map_rows(&mv, a.vp, rows, a.hd, box);
+  if (e) return e;
+  const int G = ctas(a, sms), NR = rows_of((int64_t)a.S * a.rep);
+  Params p;
+  p.a = a;
+  p.meta = static_cast<Meta*>(workspace);
+  p.part_o = reinterpret_cast<float*>(p.meta + G);
+  p.part_ml = p.part_o + (int64_t)G * 2 * NR * a.hd;
+  return a.hd == 128 ? pick<128>(mk, mv, p, G, NR, stream, launches) : pick<64>(mk, mv, p, G, NR, stream, launches);
+}
+
+int paged8_decode_error(bool reset) {
+  int h = 0;
+  if (cudaMemcpyFromSymbol(&h, p8dec::g_error, sizeof(int)) != cudaSuccess) return -1;
+  if (reset && h) {
+    const int z = 0;
+    cudaMemcpyToSymbol(p8dec::g_error, &z, sizeof(int));
+  }
+  return h;
+}
+
+}  // namespace vo

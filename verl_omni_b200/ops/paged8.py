@@ -11,7 +11,7 @@ Keys and values are e4m3 numbers with one power-of-two scale per (page, KV head)
 * :class:`PagedKVCache8` / :class:`PagedBatch8` / :class:`Paged8View` -- pools of all layers, a host block manager with
   shared (reference-counted) pages, and what one model layer receives as its cache.
 
-CUDA tensors run ``csrc/paged8.cu``; CPU tensors an fp32 torch oracle.
+CUDA tensors run ``csrc/paged8.cu`` (and the tcgen05 kernels next to it); CPU tensors an fp32 torch oracle.
 Counterpart of vLLM's fp8 ``kv_cache_dtype`` and block manager under the reference's AR rollout
 (``verl_omni/workers/rollout/vllm_rollout/vllm_omni_async_server.py:537-579``).
 """
