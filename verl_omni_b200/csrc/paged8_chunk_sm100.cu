@@ -9,8 +9,12 @@
 // lazy rescale of the output (only when it grows by more than 2^8), fp32 sums.
 // Work: as in the kernel for few rows, the 128-key tiles of all (sequence, KV head, 256 rows) items form one line split
 // evenly over one CTA per SM; causal items are as long as their last row's reach; cut items are merged in key order.
-// Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-10: pages -> f16 tiles in shared memory
-// (global loads one tile ahead in registers); 11: tensor-memory allocation, MMA issue.
+// Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-11 and 12-14: K and V pages -> f16 tiles in
+// shared memory (the codes come by TMA, a tile ahead); 15: tensor-memory allocation, MMA issue.
+// The loops are kept short (few unrolled copies): five roles run at once, and with everything unrolled the warps mostly
+// waited for instructions.
+#include <type_traits>
+
 #include "dcheck.cuh"
 #include "paged8.cuh"
 #include "paged8_tc.h"
@@ -23,9 +27,9 @@ using namespace tc8;
 using p8::AttendArgs;
 
 constexpr int TK = 128, TR = 128, ROWS = 2 * TR;
-constexpr int NTHREADS = 384;         // 12 warps: three per scheduler, 168 registers a thread
-constexpr int NLOAD = 96;             // threads that load and convert
-constexpr int KST = 2, VST = 2;       // K and V tiles in shared memory
+constexpr int NTHREADS = 512;         // 16 warps of 128 registers
+constexpr int NLK = 128, NLV = 96;    // threads that load and convert K, V
+constexpr int KST = 1, VST = 2;       // f16 K and V tiles: a K tile is free for the next one once its scores are computed
 constexpr int kSegs = 4;              // buffers of per-item values between the loaders and the softmax
 constexpr float kLazy = 8.f;          // log2 growth of the maximum that is left in the probabilities
 
@@ -36,12 +40,15 @@ struct Cfg {
   static constexpr int TILE = TK * HD * 2;  // f16 K, V or Q tile: HD / 64 groups of 64 columns, 128 rows of 128 bytes
   static constexpr int K_OFF = 2 * TILE;
   static constexpr int V_OFF = K_OFF + KST * TILE;
-  static constexpr int NAN_OFF = V_OFF + VST * TILE;  // [kSegs][HD] first key with a NaN value per column
-  static constexpr int REF_OFF = NAN_OFF + kSegs * HD * 4;  // [kSegs][2] largest scales, then 2 x 4 partial maxima
-  static constexpr int BAR_OFF = REF_OFF + kSegs * 8 + 32;
-  static constexpr int NBARS = 2 * KST + 2 * VST + 8 + 2 * kSegs;
+  static constexpr int RAW = TK * HD;
+  static constexpr int RAW_OFF = V_OFF + VST * TILE;
+  static constexpr int NAN_OFF = RAW_OFF + 2 * RAW;  // [kSegs][HD] first key with a NaN value per column
+  static constexpr int REF_OFF = NAN_OFF + kSegs * HD * 4;  // [kSegs][2] largest scales, then 4 + 4 partial maxima
+  static constexpr int QUP_OFF = REF_OFF + kSegs * 8 + 32;  // [ROWS] row factors of the queries
+  static constexpr int BAR_OFF = QUP_OFF + ROWS * 4;
+  static constexpr int NBARS = 2 * KST + 2 * VST + 8 + 2 * kSegs + 2;
   static constexpr int START_OFF = BAR_OFF + NBARS * 8;  // tmem slot, abort flag, start item, scan sums
-  static constexpr int BYTES = START_OFF + 24 + 8 * 12 + 1024;
+  static constexpr int BYTES = START_OFF + 24 + 8 * 16 + 1024;
 };
 
 struct Meta {
@@ -90,7 +97,21 @@ __device__ __forceinline__ int row_lim(const AttendArgs& a, const Walk& w, int64
   return s < w.nq ? max(0, w.len - w.nq + s + 1) : 0;
 }
 
-__device__ __forceinline__ void loader_sync() { asm volatile("bar.sync 1, 96;" ::: "memory"); }
+// 16 bytes, or zeros without an access
+__device__ __forceinline__ uint4 load16(const void* p, bool ok) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((int)ok));
+  return v;
+}
+template <bool V>
+__device__ __forceinline__ void loader_sync() {
+  if (V) asm volatile("bar.sync 2, 96;" ::: "memory");
+  else asm volatile("bar.sync 1, 128;" ::: "memory");
+}
 __device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -98,29 +119,6 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 }
 // kind::f16 instruction descriptor with f16 operands, fp32 accumulation
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn, int b_mn) { return idesc(M, N, a_mn, b_mn); }
-__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(acc));
-}
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc));
-}
-__device__ __forceinline__ void ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
-        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -155,28 +153,31 @@ __device__ __forceinline__ void fadd2(float& s0, float& s1, float a0, float a1) 
 }
 
 template <int HD>
-__global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(NTHREADS, 1)
+    chunk8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params p) {
   using C = Cfg<HD>;
   constexpr uint32_t TMEM_COLS = 512, S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
-  uint64_t* k_full = bars;              // [KST] f16 K tile written (NLOAD)
+  uint64_t* k_full = bars;              // [KST] f16 K tile written (NLK)
   uint64_t* k_empty = k_full + KST;     // [KST] its products done (commit)
-  uint64_t* v_full = k_empty + KST;     // [VST]
+  uint64_t* v_full = k_empty + KST;     // [VST] the same of V (NLV)
   uint64_t* v_empty = v_full + VST;     // [VST]
   uint64_t* s_full = v_empty + VST;     // [2] scores of a row tile (commit)
   uint64_t* p_full = s_full + 2;        // [2] probabilities written (4 warps)
   uint64_t* o_final = p_full + 2;       // [2] last product of an item done (commit)
   uint64_t* q_full = o_final + 2;       // [2] queries written (128)
-  uint64_t* ref_full = q_full + 2;      // [kSegs] largest scales of an item known (NLOAD)
-  uint64_t* nan_full = ref_full + kSegs;  // [kSegs] all its tiles loaded (NLOAD)
+  uint64_t* ref_full = q_full + 2;      // [kSegs] largest scales of an item known (NLK + NLV)
+  uint64_t* nan_full = ref_full + kSegs;  // [kSegs] all its tiles loaded (NLV)
+  uint64_t* raw_fulls = nan_full + kSegs;  // [2] codes of K, V landed (1 + tx)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::START_OFF);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 2);                      // b, kh, rt, tile
-  long long* sums = reinterpret_cast<long long*>(sm + C::START_OFF + 24);  // [12]
+  long long* sums = reinterpret_cast<long long*>(sm + C::START_OFF + 24);  // [16]
   int* nan_at = reinterpret_cast<int*>(sm + C::NAN_OFF);
   float* refs = reinterpret_cast<float*>(sm + C::REF_OFF);
+  float* q_up = reinterpret_cast<float*>(sm + C::QUP_OFF);
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int64_t R = (int64_t)a.S * a.rep;
@@ -199,14 +200,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
   }
   if (lane == 31) sums[warp] = upto;
   if (tid == 0) {
-    for (int i = 0; i < KST; ++i) mbar_init(&k_full[i], NLOAD), mbar_init(&k_empty[i], 1);
-    for (int i = 0; i < VST; ++i) mbar_init(&v_full[i], NLOAD), mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < KST; ++i) mbar_init(&k_full[i], NLK), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < VST; ++i) mbar_init(&v_full[i], NLV), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_final[i], 1), mbar_init(&q_full[i], 128);
-    for (int i = 0; i < kSegs; ++i) mbar_init(&ref_full[i], NLOAD), mbar_init(&nan_full[i], NLOAD);
+    for (int i = 0; i < kSegs; ++i) mbar_init(&ref_full[i], NLK + NLV), mbar_init(&nan_full[i], NLV);
+    for (int i = 0; i < 2; ++i) mbar_init(&raw_fulls[i], 1);
     *abort_flag = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 11) tmem_alloc(tmem_slot, TMEM_COLS);
+  if (warp == 15) tmem_alloc(tmem_slot, TMEM_COLS);
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -261,206 +265,221 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
   enter_seq(w, a);
   w.nt = tiles_of(a, w.len, w.nq, w.rt);
 
-  if (warp >= 8 && warp < 11) {
-    // ------------------------------------------------------------------ pages -> f16 tiles
-    constexpr int NC = HD / 16;                       // 16-byte pieces of a row
-    constexpr int RP = NLOAD / NC;                    // rows of a pass
-    constexpr int NI = (TK + RP - 1) / RP;            // passes: row i * RP + lt / NC, the last one partly empty
-    const int lt = tid - 256, lw = lt >> 5;
+  // ------------------------------------------------------------------ pages -> f16 tiles (K or V)
+  auto loader = [&](auto is_v) {
+    constexpr bool V = decltype(is_v)::value;
+    constexpr int NT = V ? NLV : NLK, ST = V ? VST : KST;
+    constexpr int NC = HD / 16;            // 16-byte pieces of a row
+    constexpr int RP = NT / NC;            // rows of a pass
+    constexpr int NI = (TK + RP - 1) / RP;  // passes: row i * RP + lt / NC (V: the last one partly empty)
+    const int lt = tid - (V ? 256 + NLK : 256), lw = lt >> 5;
     const int r_in = lt / NC, c = lt % NC;
-    // lane l < 16 holds the page of the tile's rows [8 l, 8 l + 8)
-    auto page_of = [&](const Walk& x) {
+    const int blk = min(a.block, TK), nblk = TK / blk;
+    const float* sc = V ? a.vs : a.ks;
+    const CUtensorMap* map = V ? &mv : &mk;
+    uint64_t *raw_full = &raw_fulls[V ? 1 : 0], *full = V ? v_full : k_full, *empty = V ? v_empty : k_empty;
+    const uint8_t* codes = sm + C::RAW_OFF + (V ? C::RAW : 0);
+    uint8_t* tiles = sm + (V ? C::V_OFF : C::K_OFF);
+    // the tile that is loaded next, by lane: rows [8 l, 8 l + 8) for lanes l and l + 16
+    int id_n = -1, off_n = 0, kh_n = 0;  // page, first row inside it, KV head
+    auto fetch = [&](const Walk& x) {
       const int t = x.tile * TK + (lane & 15) * 8;
-      return t < x.len ? __ldg(a.table + (int64_t)x.b * a.width + t / a.block) : -1;
+      kh_n = x.kh;
+      id_n = t < x.len ? __ldg(a.table + (int64_t)x.b * a.width + t / a.block) : -1;
+      off_n = t % a.block;
     };
-    auto load = [&](const uint8_t* pool, const Walk& x, int pages, uint4 (&d)[NI]) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = i * RP + r_in, t = x.tile * TK + r;
-        const int id = __shfl_sync(0xffffffffu, pages, (r >> 3) & 15);
-        const bool ok = r < TK && t < x.len && id >= 0 && id < a.pages;
-        d[i] = make_uint4(0, 0, 0, 0);
-        if (ok) d[i] = __ldg(reinterpret_cast<const uint4*>(pool + (((int64_t)id * a.Hk + x.kh) * a.block + t % a.block) * HD + c * 16));
+    auto scale_of_page = [&](int kh, int id) { return id >= 0 && id < a.pages ? __ldg(sc + (int64_t)id * a.Hk + kh) : 0.f; };
+    // starts its copies (the role's first warp, lane = page) and reads its scale; 0: no such page
+    auto start_tile = [&]() {
+      const int base = id_n >= 0 && id_n < a.pages ? (id_n * a.Hk + kh_n) * a.block + off_n : -1;
+      if (lw == 0) {
+        const int row = __shfl_sync(0xffffffffu, base, (lane * blk >> 3) & 15);
+        const bool load = lane < nblk && row >= 0;
+        const unsigned n = __popc(__ballot_sync(0xffffffffu, load));
+        if (lane == 0) mbar_expect_tx(raw_full, n * blk * HD);
+        __syncwarp();
+        if (load) tma_load_2d(smem_u32(codes) + lane * blk * HD, map, raw_full, 0, row);
       }
+      return scale_of_page(kh_n, id_n);
     };
-    // code * scale / ref in f16, 64-column groups of swizzled 128-byte rows; the two halves of a piece are written in
-    // the other order in the odd groups, so that a row's eight lanes hit different banks
-    auto store = [&](uint8_t* dst, const uint4 (&d)[NI], float scale, float inv_ref) {
-      const float mine_f = scale * inv_ref;
+    // code * scale / ref in f16, 64-column groups of swizzled 128-byte rows; rows from n on and rows without a page are
+    // zero.  The two halves of a piece are written in the other order in the odd groups, so that a row's eight lanes
+    // hit different banks.  nan: first keys with a NaN per column are noted and the value left out.
+    auto convert = [&](uint8_t* dst, int n, float factor, int* nan, int t0) {
+      const __half2 mine_f = __float2half2_rn(factor);
+      const int grp = c >> 2, i0 = (c & 3) * 2;
+      const bool odd = grp & 1;
+      uint8_t* base = dst + grp * (TK * 128);
+      constexpr int NB = 4;  // pieces in flight
+#pragma unroll 1
+      for (int b0 = 0; b0 < NI; b0 += NB) {
+        uint32_t fs[NB];
+        uint4 d[NB];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = i * RP + r_in;
-        const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, mine_f, (r >> 3) & 15));
-        if (r >= TK) break;
-        const uint32_t u[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
-        uint32_t h[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(j & 1 ? u[j >> 1] >> 16 : u[j >> 1] & 0xffff), __NV_E4M3);
-          const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f);
-          h[j] = *reinterpret_cast<const uint32_t*>(&y);
+        for (int i = 0; i < NB; ++i) {
+          const int r = (b0 + i) * RP + r_in;
+          fs[i] = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&mine_f), (r >> 3) & 15);
+          d[i] = *reinterpret_cast<const uint4*>(codes + min(r, TK - 1) * HD + c * 16);
+          if (r >= min(n, TK) || fs[i] == 0) d[i] = make_uint4(0, 0, 0, 0);
         }
-        const int grp = c >> 2, i0 = (c & 3) * 2;
-        uint8_t* base = dst + grp * (TK * 128);
-        const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
-        const bool odd = grp & 1;
-        *reinterpret_cast<uint4*>(base + swz<128>(r, odd ? i0 + 1 : i0)) = odd ? h1 : h0;
-        *reinterpret_cast<uint4*>(base + swz<128>(r, odd ? i0 : i0 + 1)) = odd ? h0 : h1;
-      }
-      fence_async_smem();
-    };
-    auto scale_of_page = [&](const float* sc, const Walk& x, int id) {
-      return id >= 0 && id < a.pages ? __ldg(sc + (int64_t)id * a.Hk + x.kh) : 0.f;
-    };
-    int seg = 0, i = 0, left = 0;
-    float kinv = 1.f, vinv = 1.f;
-    int common = 0, buf = 0;
-    int pg = ntot > 0 ? page_of(w) : -1;
-    uint4 kd[NI], vd[NI];
-    if (ntot > 0) load(a.kp, w, pg, kd);
-    for (; i < ntot; ++i) {
-      const float ksc = scale_of_page(a.ks, w, pg), vsc = scale_of_page(a.vs, w, pg);
-      load(a.vp, w, pg, vd);
-      if (left == 0) {
-        // largest scales over this item's part: the f16 numbers are relative to them
-        left = min(w.nt - w.tile, ntot - i);
-        buf = seg % kSegs;
-        const int p0 = w.tile * TK / a.block, p1 = (min(w.len, (w.tile + left) * TK) + a.block - 1) / a.block;
-        float km = 0.f, vm = 0.f;
-        for (int x = p0 + lt; x < p1; x += NLOAD) {
-          const int id = __ldg(a.table + (int64_t)w.b * a.width + x);
-          km = fmaxf(km, scale_of_page(a.ks, w, id));
-          vm = fmaxf(vm, scale_of_page(a.vs, w, id));
-        }
-        km = warp_fmax(km);
-        vm = warp_fmax(vm);
-        float* pm = refs + 2 * kSegs;
-        loader_sync();  // the maxima of the item before have been read
-        if (lane == 0) pm[lw] = km, pm[4 + lw] = vm;
-        loader_sync();
-        km = fmaxf(fmaxf(pm[0], pm[1]), pm[2]);
-        vm = fmaxf(fmaxf(pm[4], pm[5]), pm[6]);
-        km = km > 0.f ? km : 1.f;
-        vm = vm > 0.f ? vm : 1.f;
-        kinv = inv_pow2(km);
-        vinv = inv_pow2(vm);
-        common = max(1, w.len - w.nq + (int)((int64_t)w.rt * ROWS / a.rep) + 1);  // keys below: seen by every row that sees any
-        // buffers seg % kSegs were last read three items ago: this wait (two tiles back) is past that
-        mbar_wait(&k_empty[i % KST], ((i / KST) & 1) ^ 1, abort_flag, &g_error, 21);
-        for (int x = lt; x < HD; x += NLOAD) nan_at[buf * HD + x] = 0x7fffffff;
-        if (lt == 0) refs[buf * 2] = km, refs[buf * 2 + 1] = vm;
-        loader_sync();
-        mbar_arrive(&ref_full[buf]);
-        ++seg;
-      }
-      const Walk cur = w;
-      if (--left == 0) next_item(w, p);
-      else ++w.tile;
-      const int pg_next = i + 1 < ntot ? page_of(w) : -1;
-      mbar_wait(&k_empty[i % KST], ((i / KST) & 1) ^ 1, abort_flag, &g_error, 22);
-      store(sm + C::K_OFF + (i % KST) * C::TILE, kd, ksc, kinv);
-      mbar_arrive(&k_full[i % KST]);
-      if (i + 1 < ntot) load(a.kp, w, pg_next, kd);
-      if ((cur.tile + 1) * TK > common) {
-        // some row sees only part of this tile: a NaN value must not reach it through 0 * NaN
+        if (V && nan != nullptr) {
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-          uint32_t* u = reinterpret_cast<uint32_t*>(&vd[j]);
-          const int t = cur.tile * TK + j * RP + r_in;
+          for (int i = 0; i < NB; ++i) {
+            uint32_t* u = reinterpret_cast<uint32_t*>(&d[i]);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if ((((u[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0) continue;
-            for (int by = 0; by < 4; ++by)
-              if (((u[q] >> (8 * by)) & 0x7f) == 0x7f) {
-                atomicMin(&nan_at[buf * HD + c * 16 + q * 4 + by], t);
-                u[q] &= ~(0xffu << (8 * by));
-              }
-          }
-        }
-      }
-      mbar_wait(&v_empty[i % VST], ((i / VST) & 1) ^ 1, abort_flag, &g_error, 23);
-      store(sm + C::V_OFF + (i % VST) * C::TILE, vd, vsc, vinv);
-      mbar_arrive(&v_full[i % VST]);
-      if (left == 0) mbar_arrive(&nan_full[buf]);
-      pg = pg_next;
-    }
-  } else if (warp == 11) {
-    // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t id_s = idesc_f16(128, 128, 0, 0), id_o = idesc_f16(128, HD, 0, 1);
-      const uint32_t base = smem_u32(sm);
-      uint64_t* last_bar = nullptr;
-      uint32_t last_par = 0;
-      auto track = [&](uint64_t* b, uint32_t par) {
-        commit(b);
-        last_bar = b;
-        last_par = par;
-      };
-      int ns[2] = {0, 0}, nq[2] = {0, 0};  // score tiles and items issued per row tile
-      auto issue_s = [&](int t, int i) {
-        const uint32_t qa = base + t * C::TILE, ka = base + C::K_OFF + (i % KST) * C::TILE;
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (TK * 128) + (kk & 3) * 32;
-          mma_f16_ss(tmem + S_COL + t * 128, desc<128>(qa + off, 16, 1024), desc<128>(ka + off, 16, 1024), id_s, kk > 0);
-        }
-        track(&s_full[t], ns[t] & 1);
-        ++ns[t];
-      };
-      auto issue_pv = [&](int t, int i, bool first) {
-        const uint32_t va = base + C::V_OFF + (i % VST) * C::TILE;
-#pragma unroll
-        for (int kk = 0; kk < TK / 16; ++kk)
-          mma_f16_ts(tmem + O_COL + t * HD, tmem + S_COL + t * 128 + kk * 8, desc<128>(va + kk * 2048, TK * 128, 1024), id_o,
-                     !first || kk > 0);
-      };
-      bool ok = true;
-      int i = 0;
-      while (ok && i < ntot) {
-        const int n = min(w.nt - w.tile, ntot - i);
-        const bool two = (int64_t)w.rt * ROWS + TR < R;
-        ok = mbar_wait(&q_full[0], nq[0] & 1, abort_flag, &g_error, 31);
-        if (ok && two) ok = mbar_wait(&q_full[1], nq[1] & 1, abort_flag, &g_error, 32);
-        ok = ok && mbar_wait(&k_full[i % KST], (i / KST) & 1, abort_flag, &g_error, 33);
-        if (!ok) break;
-        fence_after();
-        issue_s(0, i);
-        if (two) issue_s(1, i);
-        track(&k_empty[i % KST], (i / KST) & 1);
-        for (int j = 0; ok && j < n; ++j, ++i) {
-          const bool more = j + 1 < n;
-          ok = mbar_wait(&v_full[i % VST], (i / VST) & 1, abort_flag, &g_error, 34) &&
-               mbar_wait(&p_full[0], (ns[0] - 1) & 1, abort_flag, &g_error, 35);
-          if (!ok) break;
-          fence_after();
-          issue_pv(0, i, j == 0);
-          if (!two) track(&v_empty[i % VST], (i / VST) & 1);
-          if (more) {
-            ok = mbar_wait(&k_full[(i + 1) % KST], ((i + 1) / KST) & 1, abort_flag, &g_error, 36);
-            if (!ok) break;
-            fence_after();
-            issue_s(0, i + 1);
-            if (!two) track(&k_empty[(i + 1) % KST], ((i + 1) / KST) & 1);
-          } else {
-            track(&o_final[0], nq[0] & 1);
-          }
-          if (two) {
-            // (ns[1] - 1): the score tile whose probabilities these are
-            ok = mbar_wait(&p_full[1], (ns[1] - 1) & 1, abort_flag, &g_error, 37);
-            if (!ok) break;
-            fence_after();
-            issue_pv(1, i, j == 0);
-            track(&v_empty[i % VST], (i / VST) & 1);
-            if (more) {
-              issue_s(1, i + 1);
-              track(&k_empty[(i + 1) % KST], ((i + 1) / KST) & 1);
-            } else {
-              track(&o_final[1], nq[1] & 1);
+            for (int q = 0; q < 4; ++q) {
+              if ((((u[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0) continue;
+              for (int by = 0; by < 4; ++by)
+                if (((u[q] >> (8 * by)) & 0x7f) == 0x7f) {
+                  atomicMin(&nan[c * 16 + q * 4 + by], t0 + (b0 + i) * RP + r_in);
+                  u[q] &= ~(0xffu << (8 * by));
+                }
             }
           }
         }
-        ++nq[0];
-        if (two) ++nq[1];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int r = (b0 + i) * RP + r_in;
+          const uint32_t u[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+          const __half2 f = *reinterpret_cast<const __half2*>(&fs[i]);
+          uint32_t h[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const __half2_raw x = __nv_cvt_fp8x2_to_halfraw2((uint16_t)(j & 1 ? u[j >> 1] >> 16 : u[j >> 1] & 0xffff), __NV_E4M3);
+            const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x), f);
+            h[j] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+          const uint4 h0 = make_uint4(h[0], h[1], h[2], h[3]), h1 = make_uint4(h[4], h[5], h[6], h[7]);
+          if (r < TK) {
+            *reinterpret_cast<uint4*>(base + swz<128>(r, odd ? i0 + 1 : i0)) = odd ? h1 : h0;
+            *reinterpret_cast<uint4*>(base + swz<128>(r, odd ? i0 : i0 + 1)) = odd ? h0 : h1;
+          }
+        }
+      }
+      fence_async_smem();
+    };
+    int seg = 0, left = 0, common = 0, buf = 0;
+    float inv_ref = 1.f, s0 = 0.f;
+    if (ntot > 0) {
+      fetch(w);
+      s0 = start_tile();
+    }
+    for (int i = 0; i < ntot; ++i) {
+      if (left == 0) {
+        // largest scale over this item's part: the f16 numbers are relative to it
+        left = min(w.nt - w.tile, ntot - i);
+        buf = seg % kSegs;
+        const int p0 = w.tile * TK / a.block, p1 = (min(w.len, (w.tile + left) * TK) + a.block - 1) / a.block;
+        float m = 0.f;
+        for (int x = p0 + lt; x < p1; x += NT) m = fmaxf(m, scale_of_page(w.kh, __ldg(a.table + (int64_t)w.b * a.width + x)));
+        m = warp_fmax(m);
+        float* pm = refs + 2 * kSegs + (V ? 4 : 0);
+        loader_sync<V>();  // the maxima of the item before have been read
+        if (lane == 0) pm[lw] = m;
+        loader_sync<V>();
+        m = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], V ? 0.f : pm[3]));
+        m = m > 0.f ? m : 1.f;
+        inv_ref = inv_pow2(m);
+        common = max(1, w.len - w.nq + (int)((int64_t)w.rt * ROWS / a.rep) + 1);  // keys below: seen by every row that sees any
+        // buffers seg % kSegs were last read by the softmax at least three items ago: this wait is past that
+        mbar_wait(&empty[i % ST], ((i / ST) & 1) ^ 1, abort_flag, &g_error, V ? 26 : 21);
+        if (V)
+          for (int x = lt; x < HD; x += NT) nan_at[buf * HD + x] = 0x7fffffff;
+        if (lt == 0) refs[buf * 2 + (V ? 1 : 0)] = m;
+        loader_sync<V>();
+        mbar_arrive(&ref_full[buf]);
+        ++seg;
+      }
+      const int t0 = w.tile * TK, n = V ? w.len - t0 : TK;  // K: rows past the length too, their scores are masked
+      if (--left == 0) next_item(w, p);
+      else ++w.tile;
+      if (i + 1 < ntot) fetch(w);
+      mbar_wait(raw_full, i & 1, abort_flag, &g_error, V ? 25 : 24);
+      mbar_wait(&empty[i % ST], ((i / ST) & 1) ^ 1, abort_flag, &g_error, V ? 23 : 22);
+      // V: where some row sees only part of the tile, a NaN value must not reach it through 0 * NaN
+      convert(tiles + (i % ST) * C::TILE, n, s0 * inv_ref, V && t0 + TK > common ? nan_at + buf * HD : nullptr, t0);
+      mbar_arrive(&full[i % ST]);
+      loader_sync<V>();  // every loader has read the codes: their place is refilled
+      if (i + 1 < ntot) s0 = start_tile();
+      if (V && left == 0) mbar_arrive(&nan_full[buf]);
+    }
+    if (*abort_flag && lt == 0 && ntot > 0) mbar_drain(raw_full, (ntot - 1) & 1);  // copies in flight land before the CTA leaves
+  };
+  if (warp >= 8 && warp < 12) {
+    loader(std::false_type{});
+  } else if (warp >= 12 && warp < 15) {
+    loader(std::true_type{});
+  } else if (warp == 15) {
+    // ------------------------------------------------------------------ MMA issuer
+    {
+      const int e = lane == 0;
+      constexpr uint32_t id_s = idesc_f16(128, 128, 0, 0), id_o = idesc_f16(128, HD, 0, 1);
+      const uint32_t base = smem_u32(sm), tm = (uint32_t)uniform((int)tmem);
+      const int ntot_u = uniform(ntot);
+      uint64_t* last_bar = nullptr;
+      uint32_t last_par = 0;
+      auto track = [&](uint64_t* b, uint32_t par) {
+        commit(b, e);
+        last_bar = b;
+        last_par = par;
+      };
+      uint32_t ns = 0, nq = 0;  // parities of a row tile's score tiles and items, bit = row tile
+      const uint64_t q_desc = desc<128>(base, 16, 1024), k_desc = desc<128>(base + C::K_OFF, 16, 1024),
+                     v_desc = desc<128>(base + C::V_OFF, TK * 128, 1024);
+      auto issue_s = [&](int t, int i) {
+        const uint64_t q = q_desc + ((t * C::TILE) >> 4), k = k_desc + (((i % KST) * C::TILE) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          constexpr uint32_t kGroup = TK * 128 >> 4;  // descriptors count 16-byte units
+          const uint32_t off = (kk >> 2) * kGroup + (kk & 3) * 2;
+          mma_f16_ss(tm + S_COL + t * 128, q + off, k + off, id_s, kk > 0, e);
+        }
+        track(&s_full[t], (ns >> t) & 1);
+        ns ^= 1u << t;
+      };
+      auto issue_pv = [&](int t, int i, bool first) {
+        const uint64_t v = v_desc + (((i % VST) * C::TILE) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk)
+          mma_f16_ts(tm + O_COL + t * HD, tm + S_COL + t * 128 + kk * 8, v + kk * (2048 >> 4), id_o, !first || kk > 0, e);
+      };
+      bool ok = true;
+      int i = 0;
+      while (ok && i < ntot_u) {
+        const int n = uniform(min(w.nt - w.tile, ntot_u - i));
+        const int nt = uniform((int64_t)w.rt * ROWS + TR < R ? 2 : 1);  // row tiles with rows
+        ok = mbar_wait_warp(&k_full[i % KST], (i / KST) & 1, abort_flag, &g_error, 33);
+#pragma unroll 1
+        for (int t = 0; ok && t < nt; ++t) {
+          ok = mbar_wait_warp(&q_full[t], (nq >> t) & 1, abort_flag, &g_error, 31);
+          if (!ok) break;
+          fence_after();
+          issue_s(t, i);
+        }
+        if (!ok) break;
+        track(&k_empty[i % KST], (i / KST) & 1);
+        for (int j = 0; ok && j < n; ++j, ++i) {
+          const bool more = j + 1 < n;
+          ok = mbar_wait_warp(&v_full[i % VST], (i / VST) & 1, abort_flag, &g_error, 34);
+#pragma unroll 1
+          for (int t = 0; ok && t < nt; ++t) {
+            ok = mbar_wait_warp(&p_full[t], ((ns >> t) & 1) ^ 1, abort_flag, &g_error, 35);  // of the score tile issued last
+            if (!ok) break;
+            fence_after();
+            issue_pv(t, i, j == 0);
+            if (t + 1 == nt) track(&v_empty[i % VST], (i / VST) & 1);
+            if (more) {
+              if (t == 0) ok = mbar_wait_warp(&k_full[(i + 1) % KST], ((i + 1) / KST) & 1, abort_flag, &g_error, 36);
+              if (!ok) break;
+              fence_after();
+              issue_s(t, i + 1);
+              if (t + 1 == nt) track(&k_empty[(i + 1) % KST], ((i + 1) / KST) & 1);
+            } else {
+              track(&o_final[t], (nq >> t) & 1);
+            }
+          }
+        }
+        nq ^= nt == 2 ? 3u : 1u;
         next_item(w, p);
       }
       if (last_bar) mbar_drain(last_bar, last_par);
@@ -483,42 +502,51 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
       next_item(w, p);
       if (!active) continue;  // the second row tile holds no rows: nothing is issued for it
       const int lim_row = rr < R ? row_lim(a, cur, rr) : 0;
-      float up;
       {
-        // queries of this row in f16, times 2^-e
-        const bool has = rr < R;
-        const __nv_bfloat16* q = a.q + cur.b * a.qsb + (int64_t)(cur.kh * a.rep + (has ? (int)(rr % a.rep) : 0)) * a.qsh +
-                                 (has ? rr / a.rep : 0) * a.qss;
-        float m = 0.f;
-        bool finite = true;
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          const uint4 u = has ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
-          const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        // queries in f16, times 2^-e per row: the warp's 32 rows, HD / 8 lanes a row
+        constexpr int LPR = HD / 8, RPI = 32 / LPR;
+        const int c = lane % LPR;
+        const int64_t r0 = (int64_t)cur.rt * ROWS + t * TR + (warp & 3) * 32 + lane / LPR;
+#pragma unroll 1
+        for (int b0 = 0; b0 < LPR; b0 += 4) {
+          uint4 u[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float f0 = fabsf(__uint_as_float(x[k] << 16)), f1 = fabsf(__uint_as_float(x[k] & 0xffff0000u));
-            m = fmaxf(m, fmaxf(f0, f1));
-            finite = finite && f0 <= 3.4028234e38f && f1 <= 3.4028234e38f;
+          for (int i = 0; i < 4; ++i) {
+            const int64_t r = r0 + (b0 + i) * RPI;
+            const bool has = r < R;
+            const int64_t s = has ? r / a.rep : 0, h = cur.kh * a.rep + (has ? r % a.rep : 0);
+            u[i] = load16(a.q + cur.b * a.qsb + h * a.qsh + s * a.qss + c * 8, has);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rl = (warp & 3) * 32 + lane / LPR + (b0 + i) * RPI;  // row of the tile
+            const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+            // the bits of |q| order like the numbers; infinities and NaN lie above all finite ones
+            uint32_t mb = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mb = __vmaxu2(mb, x[k] & 0x7fff7fffu);
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) mb = __vmaxu2(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+            mb = max(mb & 0xffffu, mb >> 16);
+            const bool finite = mb < 0x7f80u;
+            const float up = !finite || mb == 0 ? 1.f : p8::scale_of(__uint_as_float(mb << 16)), inv = sgn * inv_pow2(up);
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              h[k] = finite ? pack_f16(__uint_as_float(x[k] << 16) * inv, __uint_as_float(x[k] & 0xffff0000u) * inv) : 0u;
+            *reinterpret_cast<uint4*>(sm + t * C::TILE + (c >> 3) * (TK * 128) + swz<128>(rl, c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+            // an infinity or NaN in the query: its scores are NaN
+            if (c == 0) q_up[t * TR + rl] = finite ? up : __int_as_float(0x7fffffff);
           }
         }
-        up = !finite || m == 0.f ? 1.f : p8::scale_of(m);
-        const float inv = sgn * inv_pow2(up);
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          const uint4 u = has && finite ? __ldg(reinterpret_cast<const uint4*>(q) + c) : make_uint4(0, 0, 0, 0);
-          const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-          uint32_t h[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) h[k] = pack_f16(__uint_as_float(x[k] << 16) * inv, __uint_as_float(x[k] & 0xffff0000u) * inv);
-          *reinterpret_cast<uint4*>(sm + t * C::TILE + (c >> 3) * (TK * 128) + swz<128>(row, c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        if (!finite) up = __int_as_float(0x7fffffff);  // an infinity or NaN in the query: its scores are NaN
         fence_async_smem();
         mbar_arrive(&q_full[t]);
+        __syncwarp();
       }
       mbar_wait(&ref_full[buf], ((seg - 1) / kSegs) & 1, abort_flag, &g_error, 41);
-      const float sl2 = sgn * a.scale_log2 * up * refs[buf * 2], vref = refs[buf * 2 + 1];
+      float sl2 = sgn * a.scale_log2 * q_up[t * TR + row] * refs[buf * 2];
+      if (sl2 == 0.f || lim_row == 0) sl2 = 1e-37f;  // keeps masked scores at -inf
+      const float vref = refs[buf * 2 + 1];
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j, ++ns) {
         const int t0 = (cur.tile + j) * TK;
@@ -526,33 +554,25 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
         mbar_wait(&s_full[t], ns & 1, abort_flag, &g_error, 42);
         __syncwarp();
         fence_after();
-        uint32_t x[32], y[32], c0[32], c1[32];
         float mx = -INFINITY;
-        ld32_nowait(S_t + 64, x);
-        ld32_nowait(S_t + 96, y);
-        wait_ld();
-        if (lim == TK) {
+        auto scores = [&](int g, uint32_t(&x)[32], uint32_t(&y)[32]) {  // 64 of them, -inf where the row does not see the key
+          ld_nowait(S_t + g * 64, x);
+          ld_nowait(S_t + g * 64 + 32, y);
+          wait_ld();
+          if (lim < (g + 1) * 64) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              x[i] = g * 64 + i < lim ? x[i] : 0xff800000u;
+              y[i] = g * 64 + 32 + i < lim ? y[i] : 0xff800000u;
+            }
+          }
+        };
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          uint32_t x[32], y[32];
+          scores(g, x, y);
 #pragma unroll
           for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (64 + i < lim) mx = fmaxf(mx, __uint_as_float(x[i]));
-            if (96 + i < lim) mx = fmaxf(mx, __uint_as_float(y[i]));
-          }
-        }
-        ld32_nowait(S_t, c0);
-        ld32_nowait(S_t + 32, c1);
-        wait_ld();
-        if (lim == TK) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(c0[i]), __uint_as_float(c1[i])));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i < lim) mx = fmaxf(mx, __uint_as_float(c0[i]));
-            if (32 + i < lim) mx = fmaxf(mx, __uint_as_float(c1[i]));
-          }
         }
         const float m_blk = mx * sl2;
         float alpha = 1.f;
@@ -563,10 +583,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
         }
         if (j > 0 && __any_sync(0xffffffffu, move)) {
           // O_t is quiescent: the product before these scores is complete, the next one waits for this warp
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t o[32];
-            ld32_nowait(O_t + c * 32, o);
+            ld_nowait(O_t + c * 32, o);
             wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
@@ -574,10 +594,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
           }
         }
         const float nmb = m == -INFINITY ? 0.f : -m;
-        float rs = 0.f, rs0 = 0.f, rs1 = 0.f;
-        auto emit = [&](const uint32_t(&v)[32], int c) {  // probabilities of 32 keys, f16 pairs over the scores' columns
-          uint32_t h[16];
-          if (lim == TK) {
+        float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {  // probabilities of 64 keys, f16 pairs over scores that have been read
+          uint32_t x[32], y[32];
+          scores(g, x, y);
+          auto emit = [&](uint32_t(&v)[32], uint32_t at) {
+            uint32_t h[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float x0, x1;
@@ -586,31 +609,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
               fadd2(rs0, rs1, e0, e1);
               h[i] = pack_f16(e0, e1);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = c * 32 + 2 * i;
-              const float e0 = k < lim ? ex2(fmaf(__uint_as_float(v[2 * i]), sl2, nmb)) : 0.f;
-              const float e1 = k + 1 < lim ? ex2(fmaf(__uint_as_float(v[2 * i + 1]), sl2, nmb)) : 0.f;
-              rs += e0 + e1;
-              h[i] = pack_f16(e0, e1);
-            }
-          }
-          st16(S_t + c * 16, h);
-        };
-        ld32_nowait(S_t + 64, x);
-        emit(c0, 0);
-        emit(c1, 1);  // columns [16, 32): chunk 1's own scores start at 32
-        wait_ld();
-        ld32_nowait(S_t + 96, y);
-        emit(x, 2);
-        wait_ld();
-        emit(y, 3);
+            st16(at, h);
+          };
+          emit(x, S_t + g * 32);
+          emit(y, S_t + g * 32 + 16);
+        }
         wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t]);
-        l = l * alpha + (rs + (rs0 + rs1));
+        l = l * alpha + (rs0 + rs1);
       }
       mbar_wait(&o_final[t], nitem & 1, abort_flag, &g_error, 43);
       mbar_wait(&nan_full[buf], ((seg - 1) / kSegs) & 1, abort_flag, &g_error, 44);
@@ -621,10 +629,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
       const float mul = whole ? (l == 0.f ? 0.f : vref / l) : vref;
       const int64_t slot = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * ROWS + t * TR + row;
       const int64_t orow = ((int64_t)cur.b * a.S + rr / a.rep) * a.Hq + cur.kh * a.rep + rr % a.rep;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t o[32];
-        ld32_nowait(O_t + c * 32, o);
+        ld_nowait(O_t + c * 32, o);
         wait_ld();
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
@@ -660,7 +668,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) chunk8_kernel(const __grid_consta
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 11) {
+  if (warp == 15) {
     __syncwarp();
     tmem_free(tmem, TMEM_COLS);
   }
@@ -701,10 +709,10 @@ __global__ void __launch_bounds__(256) merge8_kernel(const __grid_constant__ Par
 }
 
 template <int HD>
-int launch(const Params& p, int G, cudaStream_t stream, int* launches) {
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, cudaStream_t stream, int* launches) {
   static const cudaError_t set = cudaFuncSetAttribute(chunk8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES);
   if (set != cudaSuccess) return (int)set;
-  chunk8_kernel<HD><<<G, NTHREADS, Cfg<HD>::BYTES, stream>>>(p);
+  chunk8_kernel<HD><<<G, NTHREADS, Cfg<HD>::BYTES, stream>>>(mk, mv, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   ++*launches;
@@ -744,6 +752,13 @@ int64_t paged8_chunk_workspace(const p8::AttendArgs& a, int sms) {
 
 int paged8_chunk_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaStream_t stream, int* launches) {
   using namespace p8chk;
+  CUtensorMap mk, mv;
+  const int64_t rows = (int64_t)a.pages * a.Hk * a.block;
+  const int box = a.block < TK ? a.block : TK;
+  int e = map_rows(&mk, a.kp, rows, a.hd, box, false);
+  if (e) return e;
+  e = map_rows(&mv, a.vp, rows, a.hd, box, false);
+  if (e) return e;
   const int G = ctas(a, sms);
   Params p;
   p.a = a;
@@ -751,7 +766,7 @@ int paged8_chunk_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaS
   p.part_o = static_cast<float*>(workspace);  // 16-byte rows first
   p.part_ml = p.part_o + (int64_t)G * 2 * ROWS * a.hd;
   p.meta = reinterpret_cast<Meta*>(p.part_ml + (int64_t)G * 2 * ROWS * 2);
-  return a.hd == 128 ? launch<128>(p, G, stream, launches) : launch<64>(p, G, stream, launches);
+  return a.hd == 128 ? launch<128>(mk, mv, p, G, stream, launches) : launch<64>(mk, mv, p, G, stream, launches);
 }
 
 int paged8_chunk_error(bool reset) {

@@ -6,8 +6,8 @@
 // The e4m3 codes go from global memory to the tensor core as they are: a 128-key tile of K and V is staged by TMA, and
 // both products take it from shared memory (S^T = K Q^T: keys as M, rows as N; O^T = V^T P^T: dims as M).  The other
 // operand keeps its precision as a sum of two e4m3 numbers: q = 2^e (q_hi + q_lo) holds every bit of a bf16 query whose
-// elements lie within 2^10 of the row's largest (below that, 2^-19 of the largest), p likewise to 8 bits; two products
-// accumulate into the same fp32 columns.  Page scales stay outside: k_scale multiplies the thread's (key's) scores, the
+// elements lie within 2^10 of the row's largest (below that, 2^-19 of the largest), p likewise to 8 bits; both parts are
+// columns of one product (N = 2 x rows: the tile is read once for both) and are added when they are read.  Page scales stay outside: k_scale multiplies the thread's (key's) scores, the
 // v scales of a tile enter as p * v_scale / max(v_scale) and the maximum as a factor of the folded output.
 //
 // Work: the tiles of all (sequence, KV head) items form one line that the CTAs split evenly (two CTAs per SM, as many as
@@ -28,24 +28,26 @@ using namespace tc8;
 using p8::AttendArgs;
 
 constexpr int TK = 128;        // keys per tile
-constexpr int NB = 16;         // MMA N: query rows, zero-padded
+constexpr int MAXR = 16;       // query rows of an item at most
 constexpr int NTHREADS = 192;
 constexpr int kMaxBlocksPerTile = 16;  // pages of 8 rows
 constexpr float kPOne = 256.f;         // probabilities are held times 2^8 (e4m3 reaches 448)
 
 __device__ int g_error = 0;
 
-template <int HD>
+template <int HD, int NR>
 struct Cfg {
+  static constexpr int NP = NR < 8 ? 8 : NR;            // rows of a part
+  static constexpr int NB = 2 * NP;                     // MMA N: high parts, then low parts
   static constexpr int KV = TK * HD;                    // bytes of K or V of a tile
   static constexpr int STAGE = 2 * KV;
   static constexpr int STAGES = HD == 128 ? 3 : 6;      // 96 KB: two CTAs per SM
-  static constexpr int Q_OFF = STAGES * STAGE;          // q_hi, q_lo: NB rows of HD bytes
-  static constexpr int P_OFF = Q_OFF + 2 * NB * HD;     // two buffers of (p_hi, p_lo): NB rows of TK bytes
-  static constexpr int SC_OFF = P_OFF + 4 * NB * TK;    // per stage: k and v scale of each page
-  static constexpr int RED_OFF = SC_OFF + STAGES * 2 * kMaxBlocksPerTile * 4;  // [2][NB + 1][4] warp maxima
-  static constexpr int QS_OFF = RED_OFF + 2 * (NB + 1) * 16;                   // [2][NB] row factors
-  static constexpr int BAR_OFF = QS_OFF + 2 * NB * 4;
+  static constexpr int Q_OFF = STAGES * STAGE;          // NB rows of HD bytes
+  static constexpr int P_OFF = Q_OFF + NB * HD;         // two buffers of NB rows of TK bytes
+  static constexpr int SC_OFF = P_OFF + 2 * NB * TK;    // per stage: k and v scale of each page
+  static constexpr int RED_OFF = SC_OFF + STAGES * 2 * kMaxBlocksPerTile * 4;  // [2][MAXR + 1][4] warp maxima
+  static constexpr int QS_OFF = RED_OFF + 2 * (MAXR + 1) * 16;                 // [2][MAXR] row factors
+  static constexpr int BAR_OFF = QS_OFF + 2 * MAXR * 4;
   static constexpr int NBARS = 2 * STAGES + 11;
   static constexpr int START_OFF = BAR_OFF + NBARS * 8;  // tmem slot, abort flag, start item, scan sums
   static constexpr int BYTES = START_OFF + 96 + 1024;
@@ -86,9 +88,9 @@ __device__ __forceinline__ float inv_pow2(float x) { return __int_as_float((254 
 template <int HD, int NR, bool CAUSAL>
 __global__ void __launch_bounds__(NTHREADS, 2)
     decode8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params p) {
-  using C = Cfg<HD>;
-  constexpr int STAGES = C::STAGES;
-  constexpr uint32_t TMEM_COLS = 64, S_COL = 0, O_COL = 32;
+  using C = Cfg<HD, NR>;
+  constexpr int STAGES = C::STAGES, NP = C::NP, NB = C::NB;
+  constexpr uint32_t S_COL = 0, O_COL = 2 * NB, TMEM_COLS = 4 * NB;
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
@@ -242,34 +244,33 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     __syncwarp();
   } else if (warp == 5) {
     // ------------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    {
+      const int e = lane == 0;
       constexpr uint32_t id_s = idesc(128, NB, 0, 0);  // K (K-major) x Q (K-major)
       constexpr uint32_t id_o = idesc(128, NB, 1, 0);  // V (read MN-major) x P (K-major)
-      const uint32_t base = smem_u32(sm);
+      const uint32_t base = smem_u32(sm), tm = (uint32_t)uniform((int)tmem);
+      const int ntot_u = uniform(ntot);
       uint64_t* last_bar = nullptr;  // the latest commit: its completion covers every product issued
       uint32_t last_par = 0;
       int st_s = 0, ph_s = 0, st_o = 0, left = 0, seg = 0;
       auto issue_s = [&](int i) {
         if (left == 0) {  // first tile of an item: its queries
-          left = min(w.nt - w.tile, ntot - i);
-          if (!mbar_wait(q_full, seg & 1, abort_flag, &g_error, 2)) return false;
+          left = uniform(min(w.nt - w.tile, ntot_u - i));
+          if (!mbar_wait_warp(q_full, seg & 1, abort_flag, &g_error, 2)) return false;
           ++seg;
           next_item(w, a);
         }
         --left;
         const int sb = i & 1;
-        if (!mbar_wait(&full[st_s], ph_s, abort_flag, &g_error, 3) ||
-            !mbar_wait(&s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 4))
+        if (!mbar_wait_warp(&full[st_s], ph_s, abort_flag, &g_error, 3) ||
+            !mbar_wait_warp(&s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 4))
           return false;
         fence_after();
         const uint32_t ka = base + st_s * C::STAGE, qa = base + C::Q_OFF;
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int kk = 0; kk < HD / 32; ++kk)
-            mma_ss(tmem + S_COL + sb * NB, desc<HD>(ka + kk * 32, 16, 8 * HD), desc<HD>(qa + part * NB * HD + kk * 32, 16, 8 * HD),
-                   id_s, part + kk > 0 ? 1u : 0u);
-        commit(&s_full[sb]);
+        for (int kk = 0; kk < HD / 32; ++kk)
+          mma_ss(tm + S_COL + sb * NB, desc<HD>(ka + kk * 32, 16, 8 * HD), desc<HD>(qa + kk * 32, 16, 8 * HD), id_s, kk > 0, e);
+        commit(&s_full[sb], e);
         last_bar = &s_full[sb];
         last_par = (i >> 1) & 1;
         if (++st_s == STAGES) st_s = 0, ph_s ^= 1;
@@ -277,28 +278,25 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       };
       auto issue_pv = [&](int i) {
         const int sb = i & 1;
-        if (!mbar_wait(&p_full[sb], (i >> 1) & 1, abort_flag, &g_error, 5) ||
-            !mbar_wait(&o_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 6))
+        if (!mbar_wait_warp(&p_full[sb], (i >> 1) & 1, abort_flag, &g_error, 5) ||
+            !mbar_wait_warp(&o_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 6))
           return false;
         fence_after();
-        const uint32_t va = base + st_o * C::STAGE + C::KV, pa = base + C::P_OFF + sb * 2 * NB * TK;
+        const uint32_t va = base + st_o * C::STAGE + C::KV, pa = base + C::P_OFF + sb * NB * TK;
         // head_dim 64: the second half of the 128 lanes repeats the first (stride 0 between 64-dim groups), unused
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int kk = 0; kk < TK / 32; ++kk)
-            mma_ss(tmem + O_COL + sb * NB, desc<HD>(va + kk * 32 * HD, 0, 8 * HD), desc<128>(pa + part * NB * TK + kk * 32, 16, 1024),
-                   id_o, part + kk > 0 ? 1u : 0u);
-        commit(&o_full[sb]);
-        commit(&kv_empty[st_o]);
+        for (int kk = 0; kk < TK / 32; ++kk)
+          mma_ss(tm + O_COL + sb * NB, desc<HD>(va + kk * 32 * HD, 0, 8 * HD), desc<128>(pa + kk * 32, 16, 1024), id_o, kk > 0, e);
+        commit(&o_full[sb], e);
+        commit(&kv_empty[st_o], e);
         last_bar = &kv_empty[st_o];
         last_par = (i / STAGES) & 1;
         if (++st_o == STAGES) st_o = 0;
         return true;
       };
-      bool ok = ntot > 0 && issue_s(0);
-      for (int i = 0; i < ntot && ok; ++i) {
-        if (i + 1 < ntot) ok = issue_s(i + 1);
+      bool ok = ntot_u > 0 && issue_s(0);
+      for (int i = 0; i < ntot_u && ok; ++i) {
+        if (i + 1 < ntot_u) ok = issue_s(i + 1);
         if (ok) ok = issue_pv(i);
       }
       if (last_bar) mbar_drain(last_bar, last_par);  // before tensor memory is released
@@ -346,8 +344,8 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         for (int i = 0; i < 8; ++i) lo8[i] = f[i] - lo8[i];
         uint8_t* q = sm + C::Q_OFF + swz<HD>(r, c >> 1) + (c & 1) * 8;
         *reinterpret_cast<uint2*>(q) = hi;
-        *reinterpret_cast<uint2*>(q + NB * HD) = p8::pack_e4m3x8(lo8);
-        if (c == 0) qsc[buf * NB + r] = bad ? __int_as_float(0x7fffffff) : a.scale_log2 * up;
+        *reinterpret_cast<uint2*>(q + NP * HD) = p8::pack_e4m3x8(lo8);
+        if (c == 0) qsc[buf * MAXR + r] = bad ? __int_as_float(0x7fffffff) : a.scale_log2 * up;
       }
       fence_async_smem();
       mbar_arrive(q_full);
@@ -369,7 +367,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         m[h] = -INFINITY;
         lpart[h] = acc[h] = 0.f;
         alpha[h] = 1.f;
-        qf[h] = qsc[(seg & 1) * NB + h];
+        qf[h] = qsc[(seg & 1) * MAXR + h];
         if (CAUSAL) {
           const int s = h / a.rep;
           lim[h] = h < R && s < nq ? max(0, w.len - nq + s + 1) : 0;
@@ -382,13 +380,13 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         mbar_wait(&o_full[sb], (i >> 1) & 1, abort_flag, &g_error, 7);
         __syncwarp();
         fence_after();
-        uint32_t r[NR];
+        uint32_t r[NB];
         ld_nowait(trow + O_COL + sb * NB, r);
         wait_ld();
         fence_before();
         mbar_arrive(&o_empty[sb]);
 #pragma unroll
-        for (int h = 0; h < NR; ++h) acc[h] = fmaf(acc[h], alpha[h], __uint_as_float(r[h]) * vfac);
+        for (int h = 0; h < NR; ++h) acc[h] = fmaf(acc[h], alpha[h], (__uint_as_float(r[h]) + __uint_as_float(r[NP + h])) * vfac);
       };
       const Walk cur = w;
       next_item(w, a);
@@ -398,7 +396,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         mbar_wait(&s_full[sb], (i >> 1) & 1, abort_flag, &g_error, 9);
         __syncwarp();
         fence_after();
-        uint32_t r[NR];
+        uint32_t r[NB];
         ld_nowait(trow + S_COL + sb * NB, r);
         const float ksc = scl[(st * 2) * kMaxBlocksPerTile + my_blk];
         const bool there = t < cur.len;
@@ -407,20 +405,20 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         fence_before();
         mbar_arrive(&s_empty[sb]);
         float s[NR];
-        float* rd = red + sb * (NB + 1) * 4;
+        float* rd = red + sb * (MAXR + 1) * 4;
 #pragma unroll
         for (int h = 0; h < NR; ++h) {
           const bool seen = CAUSAL ? t < lim[h] : t < lim[0];
-          s[h] = !seen ? -INFINITY : ksc == 0.f ? 0.f : __uint_as_float(r[h]) * (ksc * qf[h]);
+          s[h] = !seen ? -INFINITY : ksc == 0.f ? 0.f : (__uint_as_float(r[h]) + __uint_as_float(r[NP + h])) * (ksc * qf[h]);
           const float v = warp_fmax(s[h]);
           if (lane == 0) rd[h * 4 + warp] = v;
         }
         {
           const float v = warp_fmax(vsc);
-          if (lane == 0) rd[NB * 4 + warp] = v;
+          if (lane == 0) rd[MAXR * 4 + warp] = v;
         }
         compute_sync();
-        const float4 v4 = *reinterpret_cast<const float4*>(rd + NB * 4);
+        const float4 v4 = *reinterpret_cast<const float4*>(rd + MAXR * 4);
         const float vmax = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
         const float vr = vmax > 0.f ? vsc * inv_pow2(vmax) * kPOne : 0.f;
         float alpha_now[NR], pv[NR];
@@ -434,7 +432,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
           m[h] = mn;
           pv[h] = e * vr;
         }
-        uint8_t* pb = sm + C::P_OFF + sb * 2 * NB * TK;
+        uint8_t* pb = sm + C::P_OFF + sb * NB * TK;
 #pragma unroll
         for (int h = 0; h < NR; h += 2) {
           const uint16_t hi = p8::float2_to_e4m3x2(pv[h], pv[h + 1]);
@@ -444,8 +442,8 @@ __global__ void __launch_bounds__(NTHREADS, 2)
           uint8_t* d1 = pb + swz<128>(h + 1, tid >> 4) + (tid & 15);
           d0[0] = (uint8_t)hi;
           d1[0] = (uint8_t)(hi >> 8);
-          d0[NB * TK] = (uint8_t)lo2;
-          d1[NB * TK] = (uint8_t)(lo2 >> 8);
+          d0[NP * TK] = (uint8_t)lo2;
+          d1[NP * TK] = (uint8_t)(lo2 >> 8);
         }
         uint8_t* vt = sm + st * C::STAGE + C::KV;
         if (!there || vsc == 0.f) {  // rows that hold nothing: zero, so that 0 * garbage stays 0
@@ -559,9 +557,9 @@ __global__ void __launch_bounds__(4 * HD) combine8_kernel(const AttendArgs a, co
 template <int HD, int NR, bool CAUSAL>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, cudaStream_t stream, int* launches) {
   static const cudaError_t set =
-      cudaFuncSetAttribute(decode8_kernel<HD, NR, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES);
+      cudaFuncSetAttribute(decode8_kernel<HD, NR, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD, NR>::BYTES);
   if (set != cudaSuccess) return (int)set;
-  decode8_kernel<HD, NR, CAUSAL><<<G, NTHREADS, Cfg<HD>::BYTES, stream>>>(mk, mv, p);
+  decode8_kernel<HD, NR, CAUSAL><<<G, NTHREADS, Cfg<HD, NR>::BYTES, stream>>>(mk, mv, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   ++*launches;
@@ -605,7 +603,7 @@ int ctas(const AttendArgs& a, int sms) {
 
 bool paged8_decode_ok(const p8::AttendArgs& a) {
   if (a.hd != 64 && a.hd != 128) return false;
-  if ((int64_t)a.S * a.rep > p8dec::NB) return false;
+  if ((int64_t)a.S * a.rep > p8dec::MAXR) return false;
   return paged8_pages_ok(a);
 }
 
@@ -619,9 +617,9 @@ int paged8_decode_launch(const p8::AttendArgs& a, void* workspace, int sms, cuda
   CUtensorMap mk, mv;
   const int64_t rows = (int64_t)a.pages * a.Hk * a.block;
   const int box = a.block < TK ? a.block : TK;
-  int e = map_rows(&mk, a.kp, rows, a.hd, box);
+  int e = map_rows(&mk, a.kp, rows, a.hd, box, true);
   if (e) return e;
-  e = map_rows(&mv, a.vp, rows, a.hd, box);
+  e = map_rows(&mv, a.vp, rows, a.hd, box, true);
   if (e) return e;
   const int G = ctas(a, sms), NR = rows_of((int64_t)a.S * a.rep);
   Params p;

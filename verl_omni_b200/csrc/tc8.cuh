@@ -53,6 +53,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t par, volatile in
   }
   return false;
 }
+// The same by a whole warp whose control flow stays uniform; and a value that is the same in all lanes, known to be so.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t par, volatile int* abort_flag, int* error, int code) {
+  const bool ok = mbar_wait(b, par, abort_flag, error, code);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 // A wait for copies or products of one's own before leaving, bounded the same way.
 __device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t par) {
   const unsigned long long t0 = clock64();
@@ -68,21 +74,30 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// D (tensor memory) (+)= A B, e4m3 operands, fp32 accumulation
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Issued by one lane (e != 0) of a warp that runs the loop as a whole: descriptors then stay in uniform registers, where
+// the instruction takes them from.  D (tensor memory) (+)= A B, fp32 accumulation; A from shared or tensor memory.
+#define VO_TC8_MMA(NAME, KIND, AREG, AOP)                                                                             \
+  __device__ __forceinline__ void NAME(uint32_t d, AREG a, uint64_t b, uint32_t idesc, uint32_t acc, int e) {         \
+    asm volatile(                                                                                                     \
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"                                  \
+        "@q tcgen05.mma.cta_group::1.kind::" KIND " [%0], " AOP ", %2, %3, p;\n\t}" ::"r"(d),                         \
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(e));                                                                \
+  }
+VO_TC8_MMA(mma_ss, "f8f6f4", uint64_t, "%1")   // e4m3
+VO_TC8_MMA(mma_f16_ss, "f16", uint64_t, "%1")  // f16
+#undef VO_TC8_MMA
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, int e) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(e));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void commit(uint64_t* b, int e) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
-}
-__device__ __forceinline__ void commit(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(b)),
+      "r"(e)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t cols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols));
@@ -109,6 +124,17 @@ __device__ __forceinline__ void ld_nowait(uint32_t taddr, uint32_t (&r)[16]) {
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void ld_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
 // Shared-memory matrix descriptor; ROW: bytes of a swizzled row, 128 or 64 (the swizzle of that width)
@@ -151,15 +177,16 @@ inline EncodeFn encode_fn() {
   }();
   return fn;
 }
-// rows x hd bytes (hd 64 or 128, row after row), boxes of whole rows, swizzle of the row's width
-inline int map_rows(CUtensorMap* m, const void* ptr, int64_t rows, int hd, int box_rows) {
+// rows x hd bytes (hd 64 or 128, row after row), boxes of whole rows; swizzled at the row's width, or as they are
+inline int map_rows(CUtensorMap* m, const void* ptr, int64_t rows, int hd, int box_rows, bool swizzled) {
   if (!encode_fn()) return (int)CUDA_ERROR_NOT_FOUND;
   cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows};
   cuuint64_t str[1] = {(cuuint64_t)hd};
   cuuint32_t box[2] = {(cuuint32_t)hd, (cuuint32_t)box_rows};
   cuuint32_t es[2] = {1, 1};
   return (int)encode_fn()(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, str, box, es,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
