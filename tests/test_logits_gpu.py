@@ -98,6 +98,26 @@ def test_process_logits(R, V, L, h64, dt):
     assert torch.equal(process_logits(x), x)
 
 
+@pytest.mark.parametrize("R,V,L", [(3, 20000, 4096), (3, 20000, 4097), (2, 9001, 12000), (1, 2200000, 500), (700, 40, 4100), (300, 1000, 40)])
+def test_long_history_wide_vocabulary_many_rows(R, V, L):
+    """Histories and vocabularies past what one row's token table holds, rows past the CTAs, and their gradient."""
+    from verl_omni_b200.ops.logits import pack_allowed, process_logits
+
+    torch.manual_seed(R + L)
+    x = (torch.randn(R, V, device="cuda") * 3).requires_grad_(True)
+    hist = (torch.rand(R, L, device="cuda") ** 4 * V).long().clamp(max=V - 1)
+    lens = torch.randint(L // 2, L + 1, (R,), device="cuda", dtype=torch.int32)
+    allowed = pack_allowed(torch.rand(1, V, device="cuda") < 0.9)
+    y = process_logits(x, hist, lens, lens // 3, repetition=1.5, presence=0.5, frequency=0.25, allowed=allowed)
+    g = torch.randn(R, V, device="cuda")
+    (dx,) = torch.autograd.grad(y, x, g)
+    pick = sorted({0, R // 2, R - 1})
+    want, d, size = _exact(x[pick], hist[pick], lens[pick], (lens // 3)[pick], None, 1.5, 0.5, 0.25, None, allowed)
+    # the frequency penalty adds count * 0.25: exact in the oracle, one rounding of the sum here
+    _close(y.detach()[pick], want, size, torch.float32)
+    _close(dx[pick], g[pick].double().cpu() * d, (g[pick].double().cpu() * d).abs(), torch.float32)
+
+
 @pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [700, 5000])
 def test_gradient(V, dt):
