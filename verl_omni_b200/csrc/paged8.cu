@@ -16,7 +16,8 @@ namespace {
 using p8::kMinExp;
 
 // ------------------------------------------------------------------------------------------------- append
-constexpr int kAppendThreads = 128;
+constexpr int kAppendMax = 256;  // threads at most
+constexpr int kHeld = 8;         // 16-byte pieces that a thread keeps in registers
 
 struct AppendArgs {
   const __nv_bfloat16 *k, *v;       // [B, Hk, S, hd], last dim contiguous
@@ -27,20 +28,30 @@ struct AppendArgs {
   int width, pages, B, Hk, S, hd, block, offset, touched;
 };
 
-// amax of the finite values among 8
-__device__ __forceinline__ float amax8(const float* f, float m) {
+// largest magnitude among 8 values as bf16 bits (of |x|: they order like the numbers), per half word
+__device__ __forceinline__ uint32_t amax_bits(const uint4& u, uint32_t m) {
+  m = __vmaxu2(m, u.x & 0x7fff7fffu);
+  m = __vmaxu2(m, u.y & 0x7fff7fffu);
+  m = __vmaxu2(m, u.z & 0x7fff7fffu);
+  return __vmaxu2(m, u.w & 0x7fff7fffu);
+}
+// the same over finite values only
+__device__ __forceinline__ uint32_t amax_finite(const uint4& u, uint32_t m) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(f[i]);
-    if (a <= 3.4028234e38f) m = fmaxf(m, a);  // false for inf and NaN
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = w[i] & 0x7fff7fffu;
+    m = __vmaxu2(m, a & ~__vcmpgeu2(a, 0x7f807f80u));
   }
   return m;
 }
 
-// One CTA per (sequence, touched page, KV head, K or V): amax of the new rows, the page's scale, then the codes.
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
-  __shared__ float red[32];
-  const int b = blockIdx.x / a.touched, t = blockIdx.x % a.touched, h = blockIdx.y;
+// One CTA per (sequence, touched page, KV head, K or V).  Bound by reading the new rows and writing their codes: the rows
+// are loaded once, all loads in flight, and kept in registers over the page's maximum (a page of more than
+// kAppendMax * kHeld pieces, 32 KB, is read a second time, from L2).
+__global__ void __launch_bounds__(kAppendMax) append_kernel(const AppendArgs a) {
+  __shared__ uint32_t red[kAppendMax / 32];
+  const int b = blockIdx.x / a.touched, t = blockIdx.x % a.touched, h = blockIdx.y, nt = blockDim.x, tid = threadIdx.x;
   const bool is_v = blockIdx.z != 0;
   const int p0 = a.start[b] + a.offset;
   const int n = a.counts ? max(0, min(a.counts[b], a.S)) : a.S;
@@ -52,32 +63,42 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
   if (lo >= hi) return;
   if (!VO_DCHECK(page < a.width)) return;                                // past the table: dropped
   const int id = a.table[(int64_t)b * a.width + page];
-  if (!VO_DCHECK(id >= 0 && id < a.pages)) return;
-  const int r0 = (int)(p0 + lo - base);                                  // rows already in the page
   const __nv_bfloat16* x = is_v ? a.v + b * a.vsb + h * a.vsh + lo * a.vss : a.k + b * a.ksb + h * a.ksh + lo * a.kss;
   const int64_t xs = is_v ? a.vss : a.kss;
+  const int upr = a.hd / 8, units = (hi - lo) * upr;
+  auto piece = [&](int u) { return __ldg(reinterpret_cast<const uint4*>(x + (u / upr) * xs + (u % upr) * 8)); };
+  uint4 held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = tid + i * nt < units ? piece(tid + i * nt) : make_uint4(0, 0, 0, 0);
+  if (!VO_DCHECK(id >= 0 && id < a.pages)) return;
+  const int r0 = (int)(p0 + lo - base);                                  // rows already in the page
   uint8_t* dst = (is_v ? a.vp : a.kp) + ((int64_t)id * a.Hk + h) * a.block * a.hd;
   float* sp = (is_v ? a.vs : a.ks) + (int64_t)id * a.Hk + h;
-  const int upr = a.hd / 8, units = (hi - lo) * upr;
-  float m = 0.f;
-  for (int u = threadIdx.x; u < units; u += kAppendThreads) {
-    float f[8];
-    unpack8(*reinterpret_cast<const bf16x8*>(x + (u / upr) * xs + (u % upr) * 8), f);
-    m = amax8(f, m);
-  }
-  m = warp_max(m);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-  __syncthreads();
-  m = red[0];
+  const float was = r0 > 0 ? *sp : 0.f;
+  auto page_max = [&](auto f) {
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 1; i < kAppendThreads / 32; ++i) m = fmaxf(m, red[i]);
-  float now = p8::scale_of(m);
+    for (int i = 0; i < kHeld; ++i) m = f(held[i], m);
+    for (int u = tid + kHeld * nt; u < units; u += nt) m = f(piece(u), m);
+    m = max(m & 0xffffu, m >> 16);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((tid & 31) == 0) red[tid >> 5] = m;
+    __syncthreads();
+    m = red[0];
+    for (int i = 1; i < nt / 32; ++i) m = max(m, red[i]);
+    return m;
+  };
+  uint32_t m = page_max([](const uint4& u, uint32_t v) { return amax_bits(u, v); });
+  if (m >= 0x7f80u) {  // an infinity or NaN among the rows: they do not count
+    __syncthreads();
+    m = page_max([](const uint4& u, uint32_t v) { return amax_finite(u, v); });
+  }
+  float now = p8::scale_of(__uint_as_float(m << 16));
   if (r0 > 0) {
-    const float was = *sp;
     now = fmaxf(was, now);
     if (now != was) {
       const float ratio = was / now;
-      for (int u = threadIdx.x; u < r0 * upr; u += kAppendThreads) {
+      for (int u = tid; u < r0 * upr; u += nt) {
         uint2* w = reinterpret_cast<uint2*>(dst + (int64_t)u * 8);
         float f[8];
         p8::unpack_e4m3x8(*w, f);
@@ -87,16 +108,19 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
       }
     }
   }
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) *sp = now;
+  if (tid == 0) *sp = now;  // every thread read the old scale before the barrier above
   const float inv = 1.f / now;
-  for (int u = threadIdx.x; u < units; u += kAppendThreads) {
+  auto put = [&](int u, const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     float f[8];
-    unpack8(*reinterpret_cast<const bf16x8*>(x + (u / upr) * xs + (u % upr) * 8), f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= inv;
-    *reinterpret_cast<uint2*>(dst + ((int64_t)(r0 + u / upr) * a.hd + (u % upr) * 8)) = p8::pack_e4m3x8(f);
-  }
+    for (int i = 0; i < 4; ++i) f[2 * i] = __uint_as_float(w[i] << 16) * inv, f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * inv;
+    *reinterpret_cast<uint2*>(dst + (int64_t)r0 * a.hd + (int64_t)u * 8) = p8::pack_e4m3x8(f);  // rows follow one another in a page
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (tid + i * nt < units) put(tid + i * nt, held[i]);
+  for (int u = tid + kHeld * nt; u < units; u += nt) put(u, piece(u));
 }
 
 // ------------------------------------------------------------------------------------------------- page copies
@@ -284,7 +308,11 @@ void paged8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Te
                const_cast<uint8_t*>(bytes_of(kp)), const_cast<uint8_t*>(bytes_of(vp)), ks.data_ptr<float>(), vs.data_ptr<float>(),
                table.data_ptr<int>(), start.data_ptr<int>(), cnt, (int)table.size(1), (int)kp.size(0), (int)B, (int)Hk, (int)S,
                (int)hd, block, (int)offset, touched};
-  append_kernel<<<dim3((unsigned)(B * touched), (unsigned)Hk, 2), kAppendThreads, 0, stream()>>>(a);
+  // as many threads as keep the new rows of a page in registers, a warp at least
+  const int64_t most = std::min<int64_t>(S, block) * (hd / 8);
+  int threads = 32;
+  while (threads < kAppendMax && most > threads * kHeld) threads *= 2;
+  append_kernel<<<dim3((unsigned)(B * touched), (unsigned)Hk, 2), threads, 0, stream()>>>(a);
   VO_CUDA_OK(cudaGetLastError());
   count_launch();
 }
