@@ -180,6 +180,8 @@ __global__ void __launch_bounds__(NTHREADS, 2)
   fence_before();
   __syncthreads();
   fence_after();
+  // the combine kernel's CTAs may take free places now; they wait for this grid's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const int ntot = (int)(g1 - g0);
   Walk w;  // a CTA without tiles walks nothing
@@ -506,51 +508,87 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       ++seg;
     }
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   fence_before();
   __syncthreads();
   fence_after();
   if (warp == 5) tmem_free(tmem, TMEM_COLS);
 }
 
-// Merges the partials of an item that CTA borders cut: block (c, row) acts where border c is the first inside its item.
-// Part 0 is slot 1 of the CTA before, the others slot 0 of CTAs c, c + 1, ...; four groups of HD threads take every
-// fourth part and are summed in a fixed order.
+// Merges the partials of an item that CTA borders cut: block c acts where border c is the first inside its item.  Part 0
+// is slot 1 of the CTA before, the others slot 0 of CTAs c, c + 1, ...; a warp takes a row (NR = 4: two warps, every other
+// part each; NR = 16: two rows one after the other), lane = HD / 32 columns, weights of 32 parts at once in the lanes.
+// The order of the sums is that of the keys.
 template <int HD, int NR>
-__global__ void __launch_bounds__(4 * HD) combine8_kernel(const AttendArgs a, const float* __restrict__ part_o,
-                                                          const float* __restrict__ part_ml, const Meta* __restrict__ meta) {
+__global__ void __launch_bounds__(256) combine8_kernel(const AttendArgs a, const float* __restrict__ part_o,
+                                                       const float* __restrict__ part_ml, const Meta* __restrict__ meta) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float so[4][HD], sl[4], smx[4];
-  const int c = blockIdx.x + 1, r = blockIdx.y, grp = threadIdx.x / HD, d = threadIdx.x % HD;
+  constexpr int V = HD / 32, WPR = NR < 8 ? 2 : 1;  // columns of a lane, warps of a row
+  __shared__ float so[8][HD], sml[8][2];
+  const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = a.S * a.rep;
   const int used = meta[0].used;
   if (c >= used) return;
   const Meta me = meta[c];
   if (!(me.begin < me.g0 && me.begin >= meta[c - 1].g0)) return;
   int last = c;  // one past the last CTA with a part
-  while (last < used && meta[last].g0 < me.end) ++last;
-  const int parts = last - c + 1;
-  auto row_of = [&](int i) -> int64_t { return i == 0 ? ((int64_t)(c - 1) * 2 + 1) * NR + r : (int64_t)(c + i - 1) * 2 * NR + r; };
-  float m = -INFINITY;
-  for (int i = grp; i < parts; i += 4) m = fmaxf(m, part_ml[row_of(i) * 2]);
-  if (d == 0) smx[grp] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
-  float l = 0.f, o = 0.f;
-#pragma unroll 4
-  for (int i = grp; i < parts; i += 4) {
-    const float w = m == -INFINITY ? 1.f : ex2(part_ml[row_of(i) * 2] - m);
-    l += part_ml[row_of(i) * 2 + 1] * w;
-    o += part_o[row_of(i) * HD + d] * w;
+  for (bool more = true; more;) {
+    const unsigned in = __ballot_sync(0xffffffffu, last + lane < used && meta[min(last + lane, used - 1)].g0 < me.end);
+    last += in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+    more = in == 0xffffffffu;
   }
-  so[grp][d] = o;
-  if (d == 0) sl[grp] = l;
-  __syncthreads();
-  if (grp == 0) {
-    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    o = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
-    const int b = me.item / a.Hk, kh = me.item % a.Hk;
-    const int64_t row = ((int64_t)b * a.S + r / a.rep) * a.Hq + kh * a.rep + r % a.rep;
-    a.out[row * HD + d] = __float2bfloat16_rn(l == 0.f ? 0.f : o / l);
+  const int parts = last - c + 1, sub = warp % WPR;
+#pragma unroll 1
+  for (int r = warp / WPR; r < NR; r += 8 / WPR) {
+    auto row_of = [&](int i) -> int64_t { return i == 0 ? ((int64_t)(c - 1) * 2 + 1) * NR + r : (int64_t)(c + i - 1) * 2 * NR + r; };
+    float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = 0.f;
+    for (int i0 = sub; i0 < parts; i0 += 32 * WPR) {
+      const int i = i0 + lane * WPR;
+      const float2 ml = r < R && i < parts ? *reinterpret_cast<const float2*>(part_ml + row_of(i) * 2) : make_float2(-INFINITY, 0.f);
+      const float mn = fmaxf(m, warp_fmax(ml.x));
+      const float al = mn == -INFINITY ? 1.f : ex2(m - mn), w = mn == -INFINITY ? 1.f : ex2(ml.x - mn);
+      float lw = ml.y * w;
+#pragma unroll
+      for (int s = 16; s > 0; s >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, s);
+      l = l * al + lw;
+      m = mn;
+#pragma unroll
+      for (int k = 0; k < V; ++k) o[k] *= al;
+      const int n = min(32, (parts - i0 + WPR - 1) / WPR);
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const float wj = __shfl_sync(0xffffffffu, w, j);
+        const float* x = part_o + row_of(i0 + j * WPR) * HD + lane * V;
+        if (r < R) {
+          if constexpr (V == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(x);
+            o[0] += v.x * wj, o[1] += v.y * wj, o[2] += v.z * wj, o[3] += v.w * wj;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(x);
+            o[0] += v.x * wj, o[1] += v.y * wj;
+          }
+        }
+      }
+    }
+    if constexpr (WPR == 2) {
+      if (lane == 0) sml[warp][0] = m, sml[warp][1] = l;
+#pragma unroll
+      for (int k = 0; k < V; ++k) so[warp][lane * V + k] = o[k];
+      __syncthreads();
+      if (sub == 0) {
+        const float m1 = sml[warp + 1][0], mn = fmaxf(m, m1);
+        const float w0 = mn == -INFINITY ? 1.f : ex2(m - mn), w1 = mn == -INFINITY ? 1.f : ex2(m1 - mn);
+        l = l * w0 + sml[warp + 1][1] * w1;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = o[k] * w0 + so[warp + 1][lane * V + k] * w1;
+      }
+    }
+    if (sub == 0 && r < R) {
+      const int b = me.item / a.Hk, kh = me.item % a.Hk;
+      const int64_t row = ((int64_t)b * a.S + r / a.rep) * a.Hq + kh * a.rep + r % a.rep;
+#pragma unroll
+      for (int k = 0; k < V; ++k) a.out[row * HD + lane * V + k] = __float2bfloat16_rn(l == 0.f ? 0.f : o[k] / l);
+    }
   }
 }
 
@@ -565,8 +603,8 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G,
   ++*launches;
   if (G == 1) return 0;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(G - 1, p.a.S * p.a.rep);
-  cfg.blockDim = dim3(4 * HD);
+  cfg.gridDim = dim3(G - 1);
+  cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -624,9 +662,9 @@ int paged8_decode_launch(const p8::AttendArgs& a, void* workspace, int sms, cuda
   const int G = ctas(a, sms), NR = rows_of((int64_t)a.S * a.rep);
   Params p;
   p.a = a;
-  p.meta = static_cast<Meta*>(workspace);
-  p.part_o = reinterpret_cast<float*>(p.meta + G);
+  p.part_o = static_cast<float*>(workspace);  // 16-byte rows first
   p.part_ml = p.part_o + (int64_t)G * 2 * NR * a.hd;
+  p.meta = reinterpret_cast<Meta*>(p.part_ml + (int64_t)G * 2 * NR * 2);
   return a.hd == 128 ? pick<128>(mk, mv, p, G, NR, stream, launches) : pick<64>(mk, mv, p, G, NR, stream, launches);
 }
 
