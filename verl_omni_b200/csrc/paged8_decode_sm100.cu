@@ -40,29 +40,32 @@ struct Cfg {
   static constexpr int NP = NR < 8 ? 8 : NR;            // rows of a part
   static constexpr int NB = 2 * NP;                     // MMA N: high parts, then low parts
   static constexpr int KV = TK * HD;                    // bytes of K or V of a tile
-  static constexpr int STAGE = 2 * KV;
-  static constexpr int STAGES = HD == 128 ? 3 : 6;      // 96 KB: two CTAs per SM
-  static constexpr int Q_OFF = STAGES * STAGE;          // NB rows of HD bytes
+  // K and V tiles in rings of their own, 96 KB, two CTAs per SM: a K tile is free as soon as its scores are computed, a V
+  // tile is held over the softmax
+  static constexpr int SK = HD == 128 ? 2 : 4, SV = HD == 128 ? 4 : 8;
+  static constexpr int V_OFF = SK * KV;
+  static constexpr int Q_OFF = V_OFF + SV * KV;         // NB rows of HD bytes
   static constexpr int P_OFF = Q_OFF + NB * HD;         // two buffers of NB rows of TK bytes
-  static constexpr int SC_OFF = P_OFF + 2 * NB * TK;    // per stage: k and v scale of each page
-  static constexpr int RED_OFF = SC_OFF + STAGES * 2 * kMaxBlocksPerTile * 4;  // [2][MAXR + 1][4] warp maxima
-  static constexpr int QS_OFF = RED_OFF + 2 * (MAXR + 1) * 16;                 // [2][MAXR] row factors
+  static constexpr int SC_OFF = P_OFF + 2 * NB * TK;    // per V tile: k and v scale of each page
+  static constexpr int TV_OFF = SC_OFF + SV * 2 * kMaxBlocksPerTile * 4;       // per V tile: largest v scale, whether a page is missing
+  static constexpr int RED_OFF = TV_OFF + SV * 16;                             // [2][4][MAXR] warp maxima
+  static constexpr int QS_OFF = RED_OFF + 2 * 4 * MAXR * 4;                    // [2][MAXR] row factors
   static constexpr int BAR_OFF = QS_OFF + 2 * MAXR * 4;
-  static constexpr int NBARS = 2 * STAGES + 11;
+  static constexpr int NBARS = 2 * SK + 2 * SV + 11;
   static constexpr int START_OFF = BAR_OFF + NBARS * 8;  // tmem slot, abort flag, start item, scan sums
   static constexpr int BYTES = START_OFF + 96 + 1024;
 };
 
-struct Meta {
-  long long g0, g1, begin, end;  // the CTA's tiles, the tiles of the item that holds g0
-  int item, used;                // used: CTAs with work (entry 0)
+// What the merge needs of border c (between CTA c - 1 and CTA c): parts > 0 where it is the first border inside an item.
+struct Border {
+  int item, parts;  // the item, the CTAs that hold parts of it
 };
 
 struct Params {
   AttendArgs a;
   float* part_o;   // [G][2][NR][HD]
   float* part_ml;  // [G][2][NR][2]
-  Meta* meta;      // [G]
+  Border* border;  // [G]
 };
 
 struct Walk {
@@ -89,14 +92,16 @@ template <int HD, int NR, bool CAUSAL>
 __global__ void __launch_bounds__(NTHREADS, 2)
     decode8_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ Params p) {
   using C = Cfg<HD, NR>;
-  constexpr int STAGES = C::STAGES, NP = C::NP, NB = C::NB;
+  constexpr int SK = C::SK, SV = C::SV, NP = C::NP, NB = C::NB;
   constexpr uint32_t S_COL = 0, O_COL = 2 * NB, TMEM_COLS = 4 * NB;
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::BAR_OFF);
-  uint64_t* full = bars;                 // [STAGES] tile landed (1 + tx)
-  uint64_t* kv_empty = full + STAGES;    // [STAGES] its PV products done (commit)
-  uint64_t* s_full = kv_empty + STAGES;  // [2] scores in tensor memory (commit)
+  uint64_t* k_full = bars;               // [SK] K tile landed (1 + tx)
+  uint64_t* k_empty = k_full + SK;       // [SK] its scores computed (commit)
+  uint64_t* v_full = k_empty + SK;       // [SV] V tile landed, scales written (1 + tx)
+  uint64_t* v_empty = v_full + SV;       // [SV] its products done (commit)
+  uint64_t* s_full = v_empty + SV;       // [2] scores in tensor memory (commit)
   uint64_t* s_empty = s_full + 2;        // [2] scores read (128)
   uint64_t* p_full = s_empty + 2;        // [2] probabilities written (128)
   uint64_t* o_full = p_full + 2;         // [2] tile output in tensor memory (commit)
@@ -107,27 +112,15 @@ __global__ void __launch_bounds__(NTHREADS, 2)
   int* start = reinterpret_cast<int*>(tmem_slot + 2);                      // b, kh, tile of the first tile
   long long* sums = reinterpret_cast<long long*>(sm + C::START_OFF + 24);  // [6] per-warp tile counts
   float* scl = reinterpret_cast<float*>(sm + C::SC_OFF);
+  float* tile_v = reinterpret_cast<float*>(sm + C::TV_OFF);
   float* red = reinterpret_cast<float*>(sm + C::RED_OFF);
   float* qsc = reinterpret_cast<float*>(sm + C::QS_OFF);
   const AttendArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
 
-  // ---- this CTA's share [g0, g1) of the line of tiles, and the item that holds g0
-  long long mine = 0;
-  const int per = (a.B + NTHREADS - 1) / NTHREADS;
-  for (int b = tid * per; b < min(a.B, (tid + 1) * per); ++b) mine += tiles_of(p8::seq_len(a, b));
-  long long upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long t = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += t;
-  }
-  if (lane == 31) sums[warp] = upto;
   if (tid == 0) {
-    for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&kv_empty[i], 1);
-    }
+    for (int i = 0; i < SK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < SV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_empty[i], 128);
@@ -144,6 +137,20 @@ __global__ void __launch_bounds__(NTHREADS, 2)
   if (warp == 5) tmem_alloc(tmem_slot, TMEM_COLS);
   if (warp < 4)  // rows past the queries and heads stay zero for the whole kernel
     for (int u = tid; u < (C::SC_OFF - C::Q_OFF) / 16; u += 128) reinterpret_cast<uint4*>(sm + C::Q_OFF)[u] = make_uint4(0, 0, 0, 0);
+  // everything above is on the chip: it may run before the kernels in front have ended
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- this CTA's share [g0, g1) of the line of tiles, and the item that holds g0
+  long long mine = 0;
+  const int per = (a.B + NTHREADS - 1) / NTHREADS;
+  for (int b = tid * per; b < min(a.B, (tid + 1) * per); ++b) mine += tiles_of(p8::seq_len(a, b));
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += t;
+  }
+  if (lane == 31) sums[warp] = upto;
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -153,10 +160,10 @@ __global__ void __launch_bounds__(NTHREADS, 2)
   }
   total *= a.Hk;
   const int used = (int)min((long long)gridDim.x, total);  // CTAs with work: one tile each at least
-  if (blockIdx.x == 0 && tid == 0) p.meta[0].used = used;
   const bool idle = (int)blockIdx.x >= used;
   const long long g0 = idle ? total : total * blockIdx.x / used, g1 = idle ? total : total * (blockIdx.x + 1) / used;
   long long lo = (before + upto - mine) * a.Hk;
+  if (idle && tid == 0) p.border[blockIdx.x] = Border{0, 0};
   if (g0 >= lo && g0 < lo + mine * a.Hk) {
     for (int b = tid * per;; ++b) {
       const int nt = tiles_of(p8::seq_len(a, b));
@@ -165,13 +172,10 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         start[0] = b;
         start[1] = kh;
         start[2] = (int)((g0 - lo) % nt);
-        const long long begin = lo + (long long)kh * nt;
-        Meta& me = p.meta[blockIdx.x];
-        me.g0 = g0;
-        me.g1 = g1;
-        me.begin = begin;
-        me.end = begin + nt;
-        me.item = b * a.Hk + kh;
+        // the item's tiles [begin, end); tile g lies in CTA ((g + 1) used - 1) / total
+        const long long begin = lo + (long long)kh * nt, end = begin + nt;
+        const int from = (int)(((begin + 1) * used - 1) / total), to = (int)((end * used - 1) / total);
+        p.border[blockIdx.x] = Border{b * a.Hk + kh, begin < g0 && from == (int)blockIdx.x - 1 ? to - from + 1 : 0};
         break;
       }
       lo += (long long)nt * a.Hk;
@@ -208,41 +212,55 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       const int64_t i = (int64_t)f.id * a.Hk + f.kh;
       return in_pool(f) ? make_float2(__ldg(a.ks + i), __ldg(a.vs + i)) : make_float2(0.f, 0.f);
     };
+    // the copies of one tile into ring place st of `full`, lane = page
+    auto issue = [&](const Pre& f, const CUtensorMap* m, uint64_t* full, uint32_t dst) {
+      const bool load = in_pool(f);
+      const unsigned n = __popc(__ballot_sync(0xffffffffu, load));
+      if (lane == 0) mbar_expect_tx(full, n * (uint32_t)blk * HD);
+      __syncwarp();
+      if (load) tma_load_2d(dst + lane * blk * HD, m, full, 0, (f.id * a.Hk + f.kh) * a.block + f.row);
+    };
+    const uint32_t base = smem_u32(sm);
     Pre f0{-2, 0, 0}, f1{-2, 0, 0};
     if (ntot > 0) fetch(f0);
     if (ntot > 1) fetch(f1);
     float2 s0 = scales(f0);
-    int st = 0, ph = 0, issued = 0;
+    if (ntot > 0) issue(f0, &mk, &k_full[0], base);
+    int issued = 0;
     for (int i = 0; i < ntot; ++i) {
       Pre f2{-2, 0, 0};
       if (i + 2 < ntot) fetch(f2);
       const float2 s1 = scales(f1);
+      if (i + 1 < ntot) {  // K a tile ahead of V: its place is free early
+        const int st = (i + 1) % SK;
+        bool ok = true;
+        if (lane == 0) ok = mbar_wait(&k_empty[st], (((i + 1) / SK) & 1) ^ 1, abort_flag, &g_error, 1);
+        if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
+        issue(f1, &mk, &k_full[st], base + st * C::KV);
+      }
+      const int st = i % SV;
       bool ok = true;
-      if (lane == 0) ok = mbar_wait(&kv_empty[st], ph ^ 1, abort_flag, &g_error, 1);
+      if (lane == 0) ok = mbar_wait(&v_empty[st], ((i / SV) & 1) ^ 1, abort_flag, &g_error, 11);
       if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
       if (lane < nblk) {
         scl[(st * 2) * kMaxBlocksPerTile + lane] = s0.x;  // 0: no such page, its rows read as zeros
         scl[(st * 2 + 1) * kMaxBlocksPerTile + lane] = s0.y;
       }
-      const bool load = in_pool(f0);
-      (void)VO_DCHECK(load || f0.id == -2);  // checked builds record a page id outside the pool
-      const unsigned n = __popc(__ballot_sync(0xffffffffu, load));
-      if (lane == 0) mbar_expect_tx(&full[st], n * 2u * blk * HD);
+      (void)VO_DCHECK(in_pool(f0) || f0.id == -2);  // checked builds record a page id outside the pool
+      const float vmax = warp_fmax(s0.y);  // 0 without a page
+      const bool missing = __any_sync(0xffffffffu, lane < nblk && !in_pool(f0));
+      if (lane == 0) tile_v[st * 4] = vmax, tile_v[st * 4 + 1] = missing ? 1.f : 0.f;
       __syncwarp();
-      if (load) {
-        const int row = (f0.id * a.Hk + f0.kh) * a.block + f0.row;
-        const uint32_t dst = smem_u32(sm) + st * C::STAGE + lane * blk * HD;
-        tma_load_2d(dst, &mk, &full[st], 0, row);
-        tma_load_2d(dst + C::KV, &mv, &full[st], 0, row);
-      }
+      issue(f0, &mv, &v_full[st], base + C::V_OFF + st * C::KV);
       issued = i + 1;
       f0 = f1;
       f1 = f2;
       s0 = s1;
-      if (++st == STAGES) st = 0, ph ^= 1;
     }
-    if (lane == 0 && *abort_flag)  // the copies in flight land before the CTA leaves
-      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_drain(&full[i % STAGES], (i / STAGES) & 1);
+    if (lane == 0 && *abort_flag) {  // the copies in flight land before the CTA leaves
+      for (int i = max(0, issued - SV); i < issued; ++i) mbar_drain(&v_full[i % SV], (i / SV) & 1);
+      for (int i = max(0, issued + 1 - SK); i < min(ntot, issued + 1); ++i) mbar_drain(&k_full[i % SK], (i / SK) & 1);
+    }
     __syncwarp();
   } else if (warp == 5) {
     // ------------------------------------------------------------------ MMA issuer
@@ -254,7 +272,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       const int ntot_u = uniform(ntot);
       uint64_t* last_bar = nullptr;  // the latest commit: its completion covers every product issued
       uint32_t last_par = 0;
-      int st_s = 0, ph_s = 0, st_o = 0, left = 0, seg = 0;
+      int left = 0, seg = 0;
       auto issue_s = [&](int i) {
         if (left == 0) {  // first tile of an item: its queries
           left = uniform(min(w.nt - w.tile, ntot_u - i));
@@ -263,37 +281,37 @@ __global__ void __launch_bounds__(NTHREADS, 2)
           next_item(w, a);
         }
         --left;
-        const int sb = i & 1;
-        if (!mbar_wait_warp(&full[st_s], ph_s, abort_flag, &g_error, 3) ||
+        const int sb = i & 1, st = i % SK;
+        if (!mbar_wait_warp(&k_full[st], (i / SK) & 1, abort_flag, &g_error, 3) ||
             !mbar_wait_warp(&s_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 4))
           return false;
         fence_after();
-        const uint32_t ka = base + st_s * C::STAGE, qa = base + C::Q_OFF;
+        const uint32_t ka = base + st * C::KV, qa = base + C::Q_OFF;
 #pragma unroll
         for (int kk = 0; kk < HD / 32; ++kk)
           mma_ss(tm + S_COL + sb * NB, desc<HD>(ka + kk * 32, 16, 8 * HD), desc<HD>(qa + kk * 32, 16, 8 * HD), id_s, kk > 0, e);
         commit(&s_full[sb], e);
-        last_bar = &s_full[sb];
-        last_par = (i >> 1) & 1;
-        if (++st_s == STAGES) st_s = 0, ph_s ^= 1;
+        commit(&k_empty[st], e);
+        last_bar = &k_empty[st];
+        last_par = (i / SK) & 1;
         return true;
       };
       auto issue_pv = [&](int i) {
-        const int sb = i & 1;
-        if (!mbar_wait_warp(&p_full[sb], (i >> 1) & 1, abort_flag, &g_error, 5) ||
+        const int sb = i & 1, st = i % SV;
+        if (!mbar_wait_warp(&v_full[st], (i / SV) & 1, abort_flag, &g_error, 12) ||
+            !mbar_wait_warp(&p_full[sb], (i >> 1) & 1, abort_flag, &g_error, 5) ||
             !mbar_wait_warp(&o_empty[sb], ((i >> 1) & 1) ^ 1, abort_flag, &g_error, 6))
           return false;
         fence_after();
-        const uint32_t va = base + st_o * C::STAGE + C::KV, pa = base + C::P_OFF + sb * NB * TK;
+        const uint32_t va = base + C::V_OFF + st * C::KV, pa = base + C::P_OFF + sb * NB * TK;
         // head_dim 64: the second half of the 128 lanes repeats the first (stride 0 between 64-dim groups), unused
 #pragma unroll
         for (int kk = 0; kk < TK / 32; ++kk)
           mma_ss(tm + O_COL + sb * NB, desc<HD>(va + kk * 32 * HD, 0, 8 * HD), desc<128>(pa + kk * 32, 16, 1024), id_o, kk > 0, e);
         commit(&o_full[sb], e);
-        commit(&kv_empty[st_o], e);
-        last_bar = &kv_empty[st_o];
-        last_par = (i / STAGES) & 1;
-        if (++st_o == STAGES) st_o = 0;
+        commit(&v_empty[st], e);
+        last_bar = &v_empty[st];
+        last_par = (i / SV) & 1;
         return true;
       };
       bool ok = ntot_u > 0 && issue_s(0);
@@ -308,29 +326,38 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     // ------------------------------------------------------------------ softmax and output (warps 0-3)
     const int R = a.S * a.rep;  // query rows of an item, <= NR
     // queries of item (b, kh): thread = 8 consecutive elements of a row; row factor 2^e * scale goes to the scores
-    auto load_q = [&](int b, int kh, int buf) {
-      constexpr int LPR = HD / 8;  // lanes per row
+    constexpr int LPR = HD / 8, QN = (NR * LPR + 127) / 128;  // lanes of a row, rows of a thread
+    uint4 qr[QN];
+    auto fetch_q = [&](int b, int kh) {
 #pragma unroll
-      for (int r = tid / LPR; r < NR; r += 128 / LPR) {
-        float f[8];
-        const int c = tid % LPR;
-        uint4 u = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < QN; ++i) {
+        const int r = tid / LPR + i * (128 / LPR);
+        qr[i] = make_uint4(0, 0, 0, 0);
         if (r < R) {
           const int s = r / a.rep, h = kh * a.rep + r % a.rep;
-          u = *reinterpret_cast<const uint4*>(a.q + b * a.qsb + h * a.qsh + s * a.qss + c * 8);
+          qr[i] = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.qsb + h * a.qsh + s * a.qss + (tid % LPR) * 8));
         }
+      }
+    };
+    auto load_q = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const int r = tid / LPR + i * (128 / LPR), c = tid % LPR;
+        if (r >= NR) break;  // whole warps
+        float f[8];
+        const uint4 u = qr[i];
         const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
         float m = 0.f;
         bool finite = true;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f[2 * i] = __uint_as_float(uw[i] << 16);
-          f[2 * i + 1] = __uint_as_float(uw[i] & 0xffff0000u);
+        for (int k = 0; k < 4; ++k) {
+          f[2 * k] = __uint_as_float(uw[k] << 16);
+          f[2 * k + 1] = __uint_as_float(uw[k] & 0xffff0000u);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          m = fmaxf(m, fabsf(f[i]));
-          finite = finite && fabsf(f[i]) <= 3.4028234e38f;
+        for (int k = 0; k < 8; ++k) {
+          m = fmaxf(m, fabsf(f[k]));
+          finite = finite && fabsf(f[k]) <= 3.4028234e38f;
         }
         if (!finite) m = INFINITY;
 #pragma unroll
@@ -354,14 +381,18 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     };
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
     const int blk = min(a.block, TK), my_blk = tid / blk;
-    int st = 0, seg = 0, it = 0;
-    if (ntot > 0) load_q(w.b, w.kh, 0);
+    int seg = 0, it = 0;
+    if (ntot > 0) {
+      fetch_q(w.b, w.kh);
+      load_q(0);
+    }
     while (it < ntot) {
       const int nseg = min(w.nt - w.tile, ntot - it), nq = p8::seq_q(a, w.b);
       const bool from_start = w.tile == 0, whole = from_start && nseg == w.nt;
       float m[NR], lpart[NR], acc[NR], alpha[NR], qf[NR];
       int lim[CAUSAL ? NR : 1];
-      float vfac = 0.f;
+      float vfac = 0.f;  // of the tile that is folded next, with alpha where its maximum grew
+      bool rescale = false;
       int nan_at = 0x7fffffff;  // first key whose value in this thread's column is NaN (tiles that a row sees partly)
       compute_sync();           // row factors of this item are written
 #pragma unroll
@@ -376,7 +407,8 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         }
       }
       if (!CAUSAL) lim[0] = nq > 0 ? w.len : 0;
-      const int common = CAUSAL ? max(1, w.len - nq + 1) : w.len;  // keys below it are seen by every row that sees any
+      // keys below it are seen by every row that sees any
+      const int common = nq == 0 ? 0 : CAUSAL ? max(1, w.len - nq + 1) : w.len;
       auto fold = [&](int i) {  // thread = head-dim column: acc = acc * alpha_i + O_i
         const int sb = i & 1;
         mbar_wait(&o_full[sb], (i >> 1) & 1, abort_flag, &g_error, 7);
@@ -388,88 +420,129 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         fence_before();
         mbar_arrive(&o_empty[sb]);
 #pragma unroll
-        for (int h = 0; h < NR; ++h) acc[h] = fmaf(acc[h], alpha[h], (__uint_as_float(r[h]) + __uint_as_float(r[NP + h])) * vfac);
+        for (int h = 0; h < NR; ++h) {
+          if (rescale) acc[h] *= alpha[h];
+          acc[h] = fmaf(__uint_as_float(r[h]) + __uint_as_float(r[NP + h]), vfac, acc[h]);
+        }
       };
       const Walk cur = w;
       next_item(w, a);
       for (int j = 0; j < nseg; ++j) {
-        const int i = it + j, sb = i & 1, t0 = (cur.tile + j) * TK, t = t0 + tid;
-        mbar_wait(&full[st], (i / STAGES) & 1, abort_flag, &g_error, 8);
+        const int i = it + j, sb = i & 1, st = i % SV, t0 = (cur.tile + j) * TK, t = t0 + tid;
+        const bool last_q = j + 1 == nseg && it + nseg < ntot;
+        if (last_q) fetch_q(w.b, w.kh);  // the next item's queries
+        mbar_wait(&v_full[st], (i / SV) & 1, abort_flag, &g_error, 8);
         mbar_wait(&s_full[sb], (i >> 1) & 1, abort_flag, &g_error, 9);
         __syncwarp();
         fence_after();
         uint32_t r[NB];
         ld_nowait(trow + S_COL + sb * NB, r);
         const float ksc = scl[(st * 2) * kMaxBlocksPerTile + my_blk];
-        const bool there = t < cur.len;
-        const float vsc = there ? scl[(st * 2 + 1) * kMaxBlocksPerTile + my_blk] : 0.f;
+        float vsc = scl[(st * 2 + 1) * kMaxBlocksPerTile + my_blk];
+        const float2 tv = *reinterpret_cast<const float2*>(tile_v + st * 4);
+        // a whole tile: every row sees all of its keys, all its pages exist
+        const bool full = t0 + TK <= common && tv.y == 0.f;
         wait_ld();
         fence_before();
         mbar_arrive(&s_empty[sb]);
         float s[NR];
-        float* rd = red + sb * (MAXR + 1) * 4;
 #pragma unroll
-        for (int h = 0; h < NR; ++h) {
-          const bool seen = CAUSAL ? t < lim[h] : t < lim[0];
-          s[h] = !seen ? -INFINITY : ksc == 0.f ? 0.f : (__uint_as_float(r[h]) + __uint_as_float(r[NP + h])) * (ksc * qf[h]);
-          const float v = warp_fmax(s[h]);
-          if (lane == 0) rd[h * 4 + warp] = v;
+        for (int h = 0; h < NR; ++h) s[h] = (__uint_as_float(r[h]) + __uint_as_float(r[NP + h])) * (ksc * qf[h]);
+        bool there = true;
+        if (!full) {
+          there = t < cur.len && ksc != 0.f;
+          if (!there) vsc = 0.f;
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const bool seen = CAUSAL ? t < lim[h] : t < lim[0];
+            s[h] = !seen ? -INFINITY : ksc == 0.f ? 0.f : s[h];
+          }
         }
-        {
-          const float v = warp_fmax(vsc);
-          if (lane == 0) rd[MAXR * 4 + warp] = v;
+        float4* rd = reinterpret_cast<float4*>(red + sb * 4 * MAXR);  // [warp][row]
+#pragma unroll
+        for (int h = 0; h < NR; h += 4) {
+          const float4 v = make_float4(warp_fmax(s[h]), warp_fmax(s[h + 1]), warp_fmax(s[h + 2]), warp_fmax(s[h + 3]));
+          if (lane == 0) rd[warp * (MAXR / 4) + h / 4] = v;
         }
         compute_sync();
-        const float4 v4 = *reinterpret_cast<const float4*>(rd + MAXR * 4);
-        const float vmax = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
-        const float vr = vmax > 0.f ? vsc * inv_pow2(vmax) * kPOne : 0.f;
-        float alpha_now[NR], pv[NR];
+        const float vr = tv.x > 0.f ? vsc * inv_pow2(tv.x) * kPOne : 0.f;
+        float mx[NR];
+        bool grown = false;
 #pragma unroll
-        for (int h = 0; h < NR; ++h) {
-          const float4 x = *reinterpret_cast<const float4*>(rd + h * 4);
-          const float mn = fmaxf(m[h], fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)));
-          alpha_now[h] = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
-          const float e = s[h] == -INFINITY ? 0.f : ex2(s[h] - mn);
-          lpart[h] = fmaf(lpart[h], alpha_now[h], e);
-          m[h] = mn;
-          pv[h] = e * vr;
+        for (int h = 0; h < NR; h += 4) {
+          float4 x = rd[h / 4];
+#pragma unroll
+          for (int w4 = 1; w4 < 4; ++w4) {
+            const float4 y = rd[w4 * (MAXR / 4) + h / 4];
+            x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y), x.z = fmaxf(x.z, y.z), x.w = fmaxf(x.w, y.w);
+          }
+          mx[h] = x.x, mx[h + 1] = x.y, mx[h + 2] = x.z, mx[h + 3] = x.w;
+        }
+#pragma unroll
+        for (int h = 0; h < NR; ++h) grown = grown || mx[h] > m[h];
+        float alpha_now[NR];
+        if (grown) {  // the same in all threads; rare once a sequence is under way
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const float mn = fmaxf(m[h], mx[h]);
+            alpha_now[h] = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
+            lpart[h] *= alpha_now[h];
+            m[h] = mn;
+          }
         }
         uint8_t* pb = sm + C::P_OFF + sb * NB * TK;
+        const int prow = tid & 15, pcol = tid >> 4;
 #pragma unroll
         for (int h = 0; h < NR; h += 2) {
-          const uint16_t hi = p8::float2_to_e4m3x2(pv[h], pv[h + 1]);
-          const float2 back = p8::e4m3x2_to_float2(hi);
-          const uint16_t lo2 = p8::float2_to_e4m3x2(pv[h] - back.x, pv[h + 1] - back.y);
-          uint8_t* d0 = pb + swz<128>(h, tid >> 4) + (tid & 15);
-          uint8_t* d1 = pb + swz<128>(h + 1, tid >> 4) + (tid & 15);
+          float e0, e1;
+          if (full) {  // m is finite, or the scores are NaN
+            e0 = ex2(s[h] - m[h]), e1 = ex2(s[h + 1] - m[h + 1]);
+          } else {
+            e0 = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
+            e1 = s[h + 1] == -INFINITY ? 0.f : ex2(s[h + 1] - m[h + 1]);
+          }
+          lpart[h] += e0;
+          lpart[h + 1] += e1;
+          // p to 8 bits: the nearest e4m3 number and the nearest one to what is left (f16 between: 11 bits)
+          const __half2 p16 = __floats2half2_rn(e0 * vr, e1 * vr);
+          const __nv_fp8x2_storage_t hi = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&p16), __NV_SATFINITE, __NV_E4M3);
+          const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3);
+          const __half2 rest = __hsub2(p16, *reinterpret_cast<const __half2*>(&back));
+          const __nv_fp8x2_storage_t lo2 = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&rest), __NV_SATFINITE, __NV_E4M3);
+          uint8_t* d0 = pb + swz<128>(h, pcol) + prow;
+          uint8_t* d1 = pb + swz<128>(h + 1, pcol) + prow;
           d0[0] = (uint8_t)hi;
           d1[0] = (uint8_t)(hi >> 8);
           d0[NP * TK] = (uint8_t)lo2;
           d1[NP * TK] = (uint8_t)(lo2 >> 8);
         }
-        uint8_t* vt = sm + st * C::STAGE + C::KV;
-        if (!there || vsc == 0.f) {  // rows that hold nothing: zero, so that 0 * garbage stays 0
+        if (!full) {
+          uint8_t* vt = sm + C::V_OFF + st * C::KV;
+          if (!there) {  // rows that hold nothing: zero, so that 0 * garbage stays 0
 #pragma unroll
-          for (int c = 0; c < HD / 16; ++c) reinterpret_cast<uint4*>(vt + tid * HD)[c] = make_uint4(0, 0, 0, 0);
-        }
-        if (CAUSAL && t0 + TK > common && tid < HD) {
-          // some row sees only part of this tile: a NaN value must not reach it through 0 * NaN
-          for (int k = 0; k < min(TK, cur.len - t0); ++k) {
-            uint8_t* v = vt + swz<HD>(k, tid >> 4) + (tid & 15);
-            if ((*v & 0x7f) == 0x7f) {
-              *v = 0;
-              nan_at = min(nan_at, t0 + k);
+            for (int c = 0; c < HD / 16; ++c) reinterpret_cast<uint4*>(vt + tid * HD)[c] = make_uint4(0, 0, 0, 0);
+          }
+          if (CAUSAL && tid < HD) {
+            // some row may see only part of this tile: a NaN value must not reach it through 0 * NaN
+            for (int k = 0; k < min(TK, cur.len - t0); ++k) {
+              uint8_t* v = vt + swz<HD>(k, tid >> 4) + (tid & 15);
+              if ((*v & 0x7f) == 0x7f) {
+                *v = 0;
+                nan_at = min(nan_at, t0 + k);
+              }
             }
           }
         }
         fence_async_smem();
         mbar_arrive(&p_full[sb]);
-        if (j + 1 == nseg && it + nseg < ntot) load_q(w.b, w.kh, (seg & 1) ^ 1);  // scores of this item are all read
+        if (last_q) load_q((seg & 1) ^ 1);  // scores of this item are all read
         if (j > 0) fold(i - 1);
+        rescale = grown;
+        if (grown) {
 #pragma unroll
-        for (int h = 0; h < NR; ++h) alpha[h] = alpha_now[h];
-        vfac = vmax * (1.f / kPOne);
-        if (++st == STAGES) st = 0;
+          for (int h = 0; h < NR; ++h) alpha[h] = alpha_now[h];
+        }
+        vfac = tv.x * (1.f / kPOne);
       }
       fold(it + nseg - 1);
       // sums over the keys' threads
@@ -479,7 +552,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         float v = lpart[h];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) red[h * 4 + warp] = v;
+        if (lane == 0) red[h * 4 + warp] = v;  // [row][warp] here
       }
       compute_sync();
       const int64_t slot = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * NR;
@@ -487,9 +560,9 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       for (int h = 0; h < NR; ++h) {
         if (h >= R) break;
         const float4 x = *reinterpret_cast<const float4*>(red + h * 4);
-        const float l = (x.x + x.y) + (x.z + x.w);
-        float o = acc[h];
+        float l = (x.x + x.y) + (x.z + x.w), o = acc[h];
         if (CAUSAL && lim[h] > nan_at) o = __int_as_float(0x7fffffff);
+        if (CAUSAL && lim[h] == 0) m[h] = -INFINITY, l = 0.f, o = 0.f;  // a row that sees nothing
         if (tid < HD) {
           if (whole) {
             const int64_t row = ((int64_t)cur.b * a.S + h / a.rep) * a.Hq + cur.kh * a.rep + h % a.rep;
@@ -520,22 +593,15 @@ __global__ void __launch_bounds__(NTHREADS, 2)
 // The order of the sums is that of the keys.
 template <int HD, int NR>
 __global__ void __launch_bounds__(256) combine8_kernel(const AttendArgs a, const float* __restrict__ part_o,
-                                                       const float* __restrict__ part_ml, const Meta* __restrict__ meta) {
+                                                       const float* __restrict__ part_ml, const Border* __restrict__ border) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   constexpr int V = HD / 32, WPR = NR < 8 ? 2 : 1;  // columns of a lane, warps of a row
   __shared__ float so[8][HD], sml[8][2];
   const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, R = a.S * a.rep;
-  const int used = meta[0].used;
-  if (c >= used) return;
-  const Meta me = meta[c];
-  if (!(me.begin < me.g0 && me.begin >= meta[c - 1].g0)) return;
-  int last = c;  // one past the last CTA with a part
-  for (bool more = true; more;) {
-    const unsigned in = __ballot_sync(0xffffffffu, last + lane < used && meta[min(last + lane, used - 1)].g0 < me.end);
-    last += in == 0xffffffffu ? 32 : __ffs(~in) - 1;
-    more = in == 0xffffffffu;
-  }
-  const int parts = last - c + 1, sub = warp % WPR;
+  const Border me = border[c];
+  if (me.parts == 0) return;
+  const int parts = me.parts, sub = warp % WPR;
 #pragma unroll 1
   for (int r = warp / WPR; r < NR; r += 8 / WPR) {
     auto row_of = [&](int i) -> int64_t { return i == 0 ? ((int64_t)(c - 1) * 2 + 1) * NR + r : (int64_t)(c + i - 1) * 2 * NR + r; };
@@ -597,21 +663,24 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G,
   static const cudaError_t set =
       cudaFuncSetAttribute(decode8_kernel<HD, NR, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD, NR>::BYTES);
   if (set != cudaSuccess) return (int)set;
-  decode8_kernel<HD, NR, CAUSAL><<<G, NTHREADS, Cfg<HD, NR>::BYTES, stream>>>(mk, mv, p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  ++*launches;
-  if (G == 1) return 0;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(G - 1);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, combine8_kernel<HD, NR>, p.a, (const float*)p.part_o, (const float*)p.part_ml, (const Meta*)p.meta);
+  cfg.stream = stream;
+  cfg.gridDim = dim3(G);
+  cfg.blockDim = dim3(NTHREADS);
+  cfg.dynamicSmemBytes = Cfg<HD, NR>::BYTES;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, decode8_kernel<HD, NR, CAUSAL>, mk, mv, p);
+  if (e != cudaSuccess) return (int)e;
+  ++*launches;
+  if (G == 1) return 0;
+  cfg.gridDim = dim3(G - 1);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, combine8_kernel<HD, NR>, p.a, (const float*)p.part_o, (const float*)p.part_ml, (const Border*)p.border);
   if (e != cudaSuccess) return (int)e;
   ++*launches;
   return 0;
@@ -647,7 +716,7 @@ bool paged8_decode_ok(const p8::AttendArgs& a) {
 
 int64_t paged8_decode_workspace(const p8::AttendArgs& a, int sms) {
   const int64_t G = p8dec::ctas(a, sms), NR = p8dec::rows_of((int64_t)a.S * a.rep);
-  return G * 2 * NR * (a.hd + 2) * 4 + G * (int64_t)sizeof(p8dec::Meta);
+  return G * 2 * NR * (a.hd + 2) * 4 + G * (int64_t)sizeof(p8dec::Border);
 }
 
 int paged8_decode_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaStream_t stream, int* launches) {
@@ -664,7 +733,7 @@ int paged8_decode_launch(const p8::AttendArgs& a, void* workspace, int sms, cuda
   p.a = a;
   p.part_o = static_cast<float*>(workspace);  // 16-byte rows first
   p.part_ml = p.part_o + (int64_t)G * 2 * NR * a.hd;
-  p.meta = reinterpret_cast<Meta*>(p.part_ml + (int64_t)G * 2 * NR * 2);
+  p.border = reinterpret_cast<Border*>(p.part_ml + (int64_t)G * 2 * NR * 2);
   return a.hd == 128 ? pick<128>(mk, mv, p, G, NR, stream, launches) : pick<64>(mk, mv, p, G, NR, stream, launches);
 }
 
