@@ -30,7 +30,7 @@ constexpr int TK = 128, TR = 128, ROWS = 2 * TR;
 constexpr int NTHREADS = 512;         // 16 warps of 128 registers
 constexpr int NLK = 128, NLV = 96;    // threads that load and convert K, V
 constexpr int KST = 1, VST = 2;       // f16 K and V tiles: a K tile is free for the next one once its scores are computed
-constexpr int kSegs = 4;              // buffers of per-item values between the loaders and the softmax
+constexpr int kSegs = 6;              // buffers of per-item values between the loaders and the softmax
 constexpr float kLazy = 8.f;          // log2 growth of the maximum that is left in the probabilities
 
 __device__ int g_error = 0;
@@ -51,9 +51,9 @@ struct Cfg {
   static constexpr int BYTES = START_OFF + 24 + 8 * 16 + 1024;
 };
 
-struct Meta {
-  long long g0, g1, begin, end;  // the CTA's tiles, the tiles of the item that holds g0
-  int b, kh, rt, used;           // used: CTAs with work (entry 0)
+// What the merge needs of border c (between CTA c - 1 and CTA c): parts > 0 where it is the first border inside an item.
+struct Border {
+  int b, kh, rt, parts;  // the item, the CTAs that hold parts of it
 };
 
 struct Params {
@@ -61,7 +61,7 @@ struct Params {
   int RT;          // row tiles (256) of a (sequence, KV head)
   float* part_o;   // [G][2][ROWS][HD]
   float* part_ml;  // [G][2][ROWS][2]
-  Meta* meta;
+  Border* border;  // [G]
 };
 
 // tiles of row tile rt of sequence b: up to the last key that its last query token sees (one masked tile where none is)
@@ -182,6 +182,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int64_t R = (int64_t)a.S * a.rep;
 
+  if (tid == 0) {
+    for (int i = 0; i < KST; ++i) mbar_init(&k_full[i], NLK), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < VST; ++i) mbar_init(&v_full[i], NLV), mbar_init(&v_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_final[i], 1), mbar_init(&q_full[i], 128);
+    for (int i = 0; i < kSegs; ++i) mbar_init(&ref_full[i], NLK + NLV), mbar_init(&nan_full[i], NLV);
+    for (int i = 0; i < 2; ++i) mbar_init(&raw_fulls[i], 1);
+    *abort_flag = 0;
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 15) tmem_alloc(tmem_slot, TMEM_COLS);
+  // everything above is on the chip: it may run before the kernels in front have ended
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
   // ---- this CTA's share of the line of tiles
   auto seq_tiles = [&](int b) {
     const int len = p8::seq_len(a, b), nq = p8::seq_q(a, b);
@@ -199,18 +214,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     if (lane >= o) upto += t;
   }
   if (lane == 31) sums[warp] = upto;
-  if (tid == 0) {
-    for (int i = 0; i < KST; ++i) mbar_init(&k_full[i], NLK), mbar_init(&k_empty[i], 1);
-    for (int i = 0; i < VST; ++i) mbar_init(&v_full[i], NLV), mbar_init(&v_empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_final[i], 1), mbar_init(&q_full[i], 128);
-    for (int i = 0; i < kSegs; ++i) mbar_init(&ref_full[i], NLK + NLV), mbar_init(&nan_full[i], NLV);
-    for (int i = 0; i < 2; ++i) mbar_init(&raw_fulls[i], 1);
-    *abort_flag = 0;
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  if (warp == 15) tmem_alloc(tmem_slot, TMEM_COLS);
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
@@ -220,10 +223,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   }
   total *= a.Hk;
   const int used = (int)min((long long)gridDim.x, total);  // CTAs with work: one tile each at least
-  if (blockIdx.x == 0 && tid == 0) p.meta[0].used = used;
   const bool idle = (int)blockIdx.x >= used;
   const long long g0 = idle ? total : total * blockIdx.x / used, g1 = idle ? total : total * (blockIdx.x + 1) / used;
   long long lo = (before + upto - mine) * a.Hk;
+  if (idle && tid == 0) p.border[blockIdx.x] = Border{0, 0, 0, 0};
   if (g0 >= lo && g0 < lo + mine * a.Hk) {
     for (int b = tid * per;; ++b) {
       const long long n = seq_tiles(b);
@@ -239,14 +242,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         start[1] = kh;
         start[2] = rt;
         start[3] = (int)(g0 - lo);
-        Meta& me = p.meta[blockIdx.x];
-        me.g0 = g0;
-        me.g1 = g1;
-        me.begin = lo;
-        me.end = lo + nt;
-        me.b = b;
-        me.kh = kh;
-        me.rt = rt;
+        // the item's tiles [lo, lo + nt); tile g lies in CTA ((g + 1) used - 1) / total
+        const int from = (int)(((lo + 1) * used - 1) / total), to = (int)(((lo + nt) * used - 1) / total);
+        p.border[blockIdx.x] = Border{b, kh, rt, lo < g0 && from == (int)blockIdx.x - 1 ? to - from + 1 : 0};
         break;
       }
       lo += n * a.Hk;
@@ -255,6 +253,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   fence_before();
   __syncthreads();
   fence_after();
+  // the merge kernel's CTAs may take free places now; they wait for this grid's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem = *tmem_slot;
   const int ntot = (int)(g1 - g0);
   Walk w;  // a CTA without tiles walks nothing
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         m = m > 0.f ? m : 1.f;
         inv_ref = inv_pow2(m);
         common = max(1, w.len - w.nq + (int)((int64_t)w.rt * ROWS / a.rep) + 1);  // keys below: seen by every row that sees any
-        // buffers seg % kSegs were last read by the softmax at least three items ago: this wait is past that
+        // buffers seg % kSegs were last read by the softmax several items ago: this wait is past that
         mbar_wait(&empty[i % ST], ((i / ST) & 1) ^ 1, abort_flag, &g_error, V ? 26 : 21);
         if (V)
           for (int x = lt; x < HD; x += NT) nan_at[buf * HD + x] = 0x7fffffff;
@@ -492,58 +492,66 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const uint32_t S_t = tmem + S_COL + t * 128 + lane_off, O_t = tmem + O_COL + t * HD + lane_off;
     const float sgn = a.scale_log2 < 0.f ? -1.f : 1.f;
     int it = 0, seg = 0, ns = 0, nitem = 0;
+    auto load_queries = [&](const Walk& x) {
+      // queries in f16, times 2^-e per row: the warp's 32 rows, HD / 8 lanes a row
+      constexpr int LPR = HD / 8, RPI = 32 / LPR;
+      const int c = lane % LPR;
+      const int r0 = x.rt * ROWS + t * TR + (warp & 3) * 32 + lane / LPR;
+#pragma unroll 1
+      for (int b0 = 0; b0 < LPR; b0 += 4) {
+        uint4 u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = r0 + (b0 + i) * RPI;
+          const bool has = r < R;
+          const int s = has ? r / a.rep : 0, h = x.kh * a.rep + (has ? r % a.rep : 0);
+          u[i] = load16(a.q + x.b * a.qsb + h * a.qsh + s * a.qss + c * 8, has);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int rl = (warp & 3) * 32 + lane / LPR + (b0 + i) * RPI;  // row of the tile
+          const uint32_t q4[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+          // the bits of |q| order like the numbers; infinities and NaN lie above all finite ones
+          uint32_t mb = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mb = __vmaxu2(mb, q4[k] & 0x7fff7fffu);
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) mb = __vmaxu2(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+          mb = max(mb & 0xffffu, mb >> 16);
+          const bool finite = mb < 0x7f80u;
+          const float up = !finite || mb == 0 ? 1.f : p8::scale_of(__uint_as_float(mb << 16)), inv = sgn * inv_pow2(up);
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            h[k] = finite ? pack_f16(__uint_as_float(q4[k] << 16) * inv, __uint_as_float(q4[k] & 0xffff0000u) * inv) : 0u;
+          *reinterpret_cast<uint4*>(sm + t * C::TILE + (c >> 3) * (TK * 128) + swz<128>(rl, c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+          // an infinity or NaN in the query: its scores are NaN
+          if (c == 0) q_up[t * TR + rl] = finite ? up : __int_as_float(0x7fffffff);
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(&q_full[t]);
+      __syncwarp();
+    };
+    // items without rows in this tile: nothing is issued for it
+    auto skip = [&] {
+      while (it < ntot && (int64_t)w.rt * ROWS + t * TR >= R) {
+        it += min(w.nt - w.tile, ntot - it);
+        ++seg;
+        next_item(w, p);
+      }
+    };
+    skip();
+    if (it < ntot) load_queries(w);
     while (it < ntot) {
-      const int n = min(w.nt - w.tile, ntot - it), buf = seg % kSegs;
+      const int n = min(w.nt - w.tile, ntot - it), item = seg, buf = item % kSegs;
       const Walk cur = w;
       const int64_t rr = (int64_t)w.rt * ROWS + t * TR + row;  // row among the (token, head) rows of the KV head
-      const bool active = (int64_t)w.rt * ROWS + t * TR < R;
       it += n;
       ++seg;
       next_item(w, p);
-      if (!active) continue;  // the second row tile holds no rows: nothing is issued for it
       const int lim_row = rr < R ? row_lim(a, cur, rr) : 0;
-      {
-        // queries in f16, times 2^-e per row: the warp's 32 rows, HD / 8 lanes a row
-        constexpr int LPR = HD / 8, RPI = 32 / LPR;
-        const int c = lane % LPR;
-        const int64_t r0 = (int64_t)cur.rt * ROWS + t * TR + (warp & 3) * 32 + lane / LPR;
-#pragma unroll 1
-        for (int b0 = 0; b0 < LPR; b0 += 4) {
-          uint4 u[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int64_t r = r0 + (b0 + i) * RPI;
-            const bool has = r < R;
-            const int64_t s = has ? r / a.rep : 0, h = cur.kh * a.rep + (has ? r % a.rep : 0);
-            u[i] = load16(a.q + cur.b * a.qsb + h * a.qsh + s * a.qss + c * 8, has);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rl = (warp & 3) * 32 + lane / LPR + (b0 + i) * RPI;  // row of the tile
-            const uint32_t x[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-            // the bits of |q| order like the numbers; infinities and NaN lie above all finite ones
-            uint32_t mb = 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mb = __vmaxu2(mb, x[k] & 0x7fff7fffu);
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) mb = __vmaxu2(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-            mb = max(mb & 0xffffu, mb >> 16);
-            const bool finite = mb < 0x7f80u;
-            const float up = !finite || mb == 0 ? 1.f : p8::scale_of(__uint_as_float(mb << 16)), inv = sgn * inv_pow2(up);
-            uint32_t h[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              h[k] = finite ? pack_f16(__uint_as_float(x[k] << 16) * inv, __uint_as_float(x[k] & 0xffff0000u) * inv) : 0u;
-            *reinterpret_cast<uint4*>(sm + t * C::TILE + (c >> 3) * (TK * 128) + swz<128>(rl, c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-            // an infinity or NaN in the query: its scores are NaN
-            if (c == 0) q_up[t * TR + rl] = finite ? up : __int_as_float(0x7fffffff);
-          }
-        }
-        fence_async_smem();
-        mbar_arrive(&q_full[t]);
-        __syncwarp();
-      }
-      mbar_wait(&ref_full[buf], ((seg - 1) / kSegs) & 1, abort_flag, &g_error, 41);
+      mbar_wait(&ref_full[buf], (item / kSegs) & 1, abort_flag, &g_error, 41);
       float sl2 = sgn * a.scale_log2 * q_up[t * TR + row] * refs[buf * 2];
       if (sl2 == 0.f || lim_row == 0) sl2 = 1e-37f;  // keeps masked scores at -inf
       const float vref = refs[buf * 2 + 1];
@@ -620,8 +628,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         if (lane == 0) mbar_arrive(&p_full[t]);
         l = l * alpha + (rs0 + rs1);
       }
+      skip();
+      if (it < ntot) load_queries(w);  // this item's scores are all computed; its last products run meanwhile
       mbar_wait(&o_final[t], nitem & 1, abort_flag, &g_error, 43);
-      mbar_wait(&nan_full[buf], ((seg - 1) / kSegs) & 1, abort_flag, &g_error, 44);
+      mbar_wait(&nan_full[buf], (item / kSegs) & 1, abort_flag, &g_error, 44);
       ++nitem;
       __syncwarp();
       fence_after();
@@ -664,7 +674,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       fence_before();
     }
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   fence_before();
   __syncthreads();
   fence_after();
@@ -678,20 +687,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 template <int HD>
 __global__ void __launch_bounds__(256) merge8_kernel(const __grid_constant__ Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const AttendArgs& a = p.a;
   const int c = blockIdx.x + 1, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int used = p.meta[0].used;
-  if (c >= used) return;
-  const Meta me = p.meta[c];
-  if (!(me.begin < me.g0 && me.begin >= p.meta[c - 1].g0)) return;
+  const Border me = p.border[c];
+  if (me.parts == 0) return;
   const int64_t rr = (int64_t)me.rt * ROWS + r;
   if (rr >= (int64_t)a.S * a.rep) return;
   constexpr int V = HD / 32;
   float m = -INFINITY;
   auto row_of = [&](int i) -> int64_t { return i == c - 1 ? ((int64_t)i * 2 + 1) * ROWS + r : (int64_t)i * 2 * ROWS + r; };
-  int last = c;
-  for (; last < used && p.meta[last].g0 < me.end; ++last) {
-  }
+  const int last = c - 1 + me.parts;
   for (int i = c - 1; i < last; ++i) m = fmaxf(m, p.part_ml[row_of(i) * 2]);
   float l = 0.f, o[V];
 #pragma unroll
@@ -712,20 +718,23 @@ template <int HD>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, cudaStream_t stream, int* launches) {
   static const cudaError_t set = cudaFuncSetAttribute(chunk8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES);
   if (set != cudaSuccess) return (int)set;
-  chunk8_kernel<HD><<<G, NTHREADS, Cfg<HD>::BYTES, stream>>>(mk, mv, p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  ++*launches;
-  if (G == 1) return 0;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(G - 1, ROWS / 8);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  cfg.stream = stream;
+  cfg.gridDim = dim3(G);
+  cfg.blockDim = dim3(NTHREADS);
+  cfg.dynamicSmemBytes = Cfg<HD>::BYTES;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, chunk8_kernel<HD>, mk, mv, p);
+  if (e != cudaSuccess) return (int)e;
+  ++*launches;
+  if (G == 1) return 0;
+  cfg.gridDim = dim3(G - 1, ROWS / 8);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&cfg, merge8_kernel<HD>, p);
   if (e != cudaSuccess) return (int)e;
   ++*launches;
@@ -747,7 +756,7 @@ bool paged8_chunk_ok(const p8::AttendArgs& a) {
 
 int64_t paged8_chunk_workspace(const p8::AttendArgs& a, int sms) {
   const int64_t G = p8chk::ctas(a, sms);
-  return G * 2 * p8chk::ROWS * (a.hd + 2) * 4 + G * (int64_t)sizeof(p8chk::Meta);
+  return G * 2 * p8chk::ROWS * (a.hd + 2) * 4 + G * (int64_t)sizeof(p8chk::Border);
 }
 
 int paged8_chunk_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaStream_t stream, int* launches) {
@@ -765,7 +774,7 @@ int paged8_chunk_launch(const p8::AttendArgs& a, void* workspace, int sms, cudaS
   p.RT = (int)row_tiles(a);
   p.part_o = static_cast<float*>(workspace);  // 16-byte rows first
   p.part_ml = p.part_o + (int64_t)G * 2 * ROWS * a.hd;
-  p.meta = reinterpret_cast<Meta*>(p.part_ml + (int64_t)G * 2 * ROWS * 2);
+  p.border = reinterpret_cast<Border*>(p.part_ml + (int64_t)G * 2 * ROWS * 2);
   return a.hd == 128 ? launch<128>(mk, mv, p, G, stream, launches) : launch<64>(mk, mv, p, G, stream, launches);
 }
 
