@@ -457,3 +457,49 @@ def test_empty_calls():
     out = attend_paged8(torch.randn(1, 4, 1, 64, device="cuda").bfloat16(), kp, vp, ks, vs, t.new_zeros(1, 0), one)
     assert not out.any()
     append_paged8(torch.zeros(0, 2, 3, 64, device="cuda").bfloat16(), torch.zeros(0, 2, 3, 64, device="cuda").bfloat16(), kp, vp, ks, vs, t, z)
+
+
+# ------------------------------------------------------------------------------------------------ rollout
+def test_rollout_graph_groups_and_chunks(monkeypatch):
+    """The thinker's rollout on the 8-bit cache: the decode step captured as a CUDA graph equals eager steps, shared
+    prompt pages equal unshared ones, and penalties and a grammar mask run in the same loop."""
+    from verl_omni_b200.models.moe_llm import MoEConfig, MoELLM
+    from verl_omni_b200.ops._ext import ext
+    from verl_omni_b200.ops.logits import pack_allowed
+    from verl_omni_b200.ops.paged8 import PagedKVCache8
+    from verl_omni_b200.utils.dataproto import DataProto
+    from verl_omni_b200.workers.rollout.llm_rollout import LLMRolloutEngine
+
+    torch.manual_seed(0)
+    cfg = MoEConfig(vocab=2048, hidden=512, layers=2, q_heads=16, kv_heads=2, head_dim=128, experts=8, top_k=2,
+                    expert_ffn=256, audio_layers=1, audio_dim=128, audio_mel=16, vision_layers=1, vision_dim=128,
+                    vision_patch_dim=48, audio_token=2046, image_token=2047)
+    m = MoELLM(cfg).to("cuda", torch.bfloat16).eval()
+    ids = torch.randint(0, 2000, (2, 37)).repeat_interleave(3, 0)
+    batch = DataProto({"input_ids": ids}, {})
+    ban = torch.ones(1, 2048, dtype=torch.bool, device="cuda")
+    ban[0, 100:] = False
+    mask = pack_allowed(ban)
+    kw = dict(max_new_tokens=40, temperature=0.0, device=torch.device("cuda"), kv_cache_dtype="fp8_e4m3", kv_block_size=16,
+              repetition_penalty=1.2, presence_penalty=0.1, frequency_penalty=0.05, allowed_tokens=lambda said: mask)
+    out = {}
+    for graph in ("0", "1"):
+        for group in (1, 3):
+            monkeypatch.setenv("VO_DECODE_GRAPH", graph)
+            out[graph, group] = LLMRolloutEngine(m, **kw).generate(batch, seed=0, group=group)
+    torch.cuda.synchronize()
+    assert ext().paged8_error(False) == 0
+    ref = out["0", 1].batch
+    assert bool((ref["responses"] < 100).all())
+    for o in out.values():
+        assert torch.equal(o.batch["responses"], ref["responses"])
+        torch.testing.assert_close(o.batch["rollout_log_probs"], ref["rollout_log_probs"], rtol=1e-4, atol=1e-4)
+    assert torch.equal(ref["responses"][0], ref["responses"][2]) and ref["responses"].shape == (6, 40)
+    # a prompt continued in chunks against the cache stays near the whole prompt's hidden states (8-bit keys and values)
+    c = PagedKVCache8(cfg.layers, 12, cfg.kv_heads, 16, cfg.head_dim, "cuda")
+    views = c.batch([c.add_sequence(), c.add_sequence()]).views()
+    p = torch.randint(0, 2000, (2, 90), device="cuda")
+    with torch.no_grad():
+        whole = m(p, return_hidden=True).float()
+        part = torch.cat([m(p[:, a:b], caches=views, pos0=a, return_hidden=True).float() for a, b in ((0, 30), (30, 89), (89, 90))], 1)
+    assert float((part - whole).norm() / whole.norm()) < 0.1

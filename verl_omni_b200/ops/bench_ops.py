@@ -479,6 +479,68 @@ def bench_decode(a) -> list[dict]:
     return out
 
 
+def bench_paged8(a) -> list[dict]:
+    """8-bit paged KV cache, Qwen3-Omni-30B-A3B thinker heads: ``--B`` sequences with ``--S`` cached rows in pages of 16 and
+    128 rows.  Attention of one new token and of a 512-token chunk (4 sequences), the append of one token and of the whole
+    prompts, page copies of all blocks' first halves onto the second."""
+    from verl_omni_b200.ops.paged8 import append_paged8, attend_paged8, copy_pages
+
+    B, L, Hk, rep, hd = a.B, a.S, 4, 8, 128
+    out = []
+    for bs in (16, 128):
+        W = -(-L // bs)
+        shape = (B * W, Hk, bs, hd)
+        kp, vp = (torch.zeros(shape, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+        ks, vs = (torch.ones(shape[:2], device="cuda") for _ in range(2))
+        table = torch.randperm(B * W, device="cuda").view(B, W).to(torch.int32)
+        zero, full = (torch.full((B,), n, dtype=torch.int32, device="cuda") for n in (0, L))
+        k, v = (torch.randn(B, Hk, L, hd, device="cuda").bfloat16() for _ in range(2))
+        q = torch.randn(B, Hk * rep, 1, hd, device="cuda").bfloat16()
+        qc = torch.randn(4, Hk * rep, 512, hd, device="cuda").bfloat16()
+        rows = 2 * B * Hk * L * hd
+        half = B * W // 2
+        src = torch.arange(half, dtype=torch.int32, device="cuda")
+        pools = [t.unsqueeze(0) for t in (kp, vp, ks, vs)]
+        for name, nbytes, flops, fn in (
+                ("append_prompts", 3 * rows, 0, lambda: append_paged8(k, v, kp, vp, ks, vs, table, zero)),
+                ("append_token", 3 * rows // L, 0, lambda: append_paged8(k[:, :, :1], v[:, :, :1], kp, vp, ks, vs, table, full - 1)),
+                ("attend_token", rows, 4 * B * L * Hk * rep * hd, lambda: attend_paged8(q, kp, vp, ks, vs, table, full)),
+                ("attend_chunk512", 0, 4 * 4 * 512 * (L - 255) * Hk * rep * hd,
+                 lambda: attend_paged8(qc, kp, vp, ks, vs, table[:4].contiguous(), full[:4].contiguous())),
+                ("copy_pages", rows, 0, lambda: copy_pages(pools, src, src + half))):
+            if a.only and name not in a.only.split(","):
+                continue
+            ms = timeit(fn, a.iters)
+            r = {"op": f"paged8_{name}", "block": bs, "B": B, "rows": L, "ms": round(ms, 4)}
+            if nbytes:
+                r["gbs"] = round(nbytes / ms / 1e6, 1)
+            if flops:
+                r["tflops"] = round(flops / ms / 1e9, 1)
+            out.append(r)
+    return out
+
+
+def bench_logits(a) -> list[dict]:
+    """Logits processing over the thinker's vocabulary: ``--B`` rows, ``--S`` history tokens each, fp32 with penalties and a
+    grammar mask, bf16 forward and backward; bytes counted as the logits read and written."""
+    from verl_omni_b200.ops.logits import process_logits
+
+    R, V, L = a.B, 151936, a.S
+    hist = (torch.rand(R, L, device="cuda").pow(4) * V).long().clamp(max=V - 1)
+    lens = torch.full((R,), L, dtype=torch.int32, device="cuda")
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (R, V // 32), device="cuda").to(torch.int32)
+    kw = dict(history=hist, lens=lens, repetition=1.1, presence=0.2, frequency=0.1)
+    x = torch.randn(R, V, device="cuda")
+    xb = x.bfloat16().requires_grad_(True)
+    g = torch.randn(R, V, device="cuda").bfloat16()
+    out = []
+    for name, nbytes, fn in (("fp32_masked", 8 * R * V, lambda: process_logits(x, allowed=allowed, **kw)),
+                             ("bf16_fwd_bwd", 8 * R * V, lambda: torch.autograd.grad(process_logits(xb, **kw), xb, g))):
+        ms = timeit(fn, a.iters)
+        out.append({"op": f"logits_{name}", "rows": R, "vocab": V, "history": L, "ms": round(ms, 4), "gbs": round(nbytes / ms / 1e6, 1)})
+    return out
+
+
 def bench_rollout_decode(a) -> list[dict]:
     """Thinker decode steps at full Qwen3-Omni-30B-A3B width (hidden 2048, 32 / 4 heads of 128, 128 experts,
     top-8, vocab 151936) with ``--layers`` layers: ``--B`` sequences, ``--S``-token prompts, greedy.  The time
@@ -593,7 +655,7 @@ def bench_groupnorm(a) -> list[dict]:
 
 def main() -> None:
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=["gemm", "gemm_sweep", "gemm_pair", "ulysses", "tp", "fmha", "sde", "adaln", "optstep", "moe", "groupnorm", "decode", "rollout_decode", "rowops"])
+    ap.add_argument("op", choices=["gemm", "gemm_sweep", "gemm_pair", "ulysses", "tp", "fmha", "sde", "adaln", "optstep", "moe", "groupnorm", "decode", "rollout_decode", "rowops", "paged8", "logits"])
     ap.add_argument("--numel", type=int, default=2_240_000_000)
     ap.add_argument("--M", type=int, default=21712)
     ap.add_argument("--N", type=int, default=6144)
@@ -609,7 +671,8 @@ def main() -> None:
     ap.add_argument("--new", type=int, default=64)
     a = ap.parse_args()
     pk = _peaks()
-    rows = {"gemm": bench_gemm, "gemm_sweep": bench_gemm_sweep, "gemm_pair": bench_gemm_pair, "ulysses": bench_ulysses, "tp": bench_tp, "fmha": bench_fmha, "optstep": bench_optstep, "sde": bench_sde, "adaln": bench_adaln, "moe": bench_moe, "groupnorm": bench_groupnorm, "decode": bench_decode, "rollout_decode": bench_rollout_decode, "rowops": bench_rowops}[a.op](a)
+    rows = {"gemm": bench_gemm, "gemm_sweep": bench_gemm_sweep, "gemm_pair": bench_gemm_pair, "ulysses": bench_ulysses, "tp": bench_tp, "fmha": bench_fmha, "optstep": bench_optstep, "sde": bench_sde, "adaln": bench_adaln, "moe": bench_moe, "groupnorm": bench_groupnorm, "decode": bench_decode, "rollout_decode": bench_rollout_decode, "rowops": bench_rowops,
+            "paged8": bench_paged8, "logits": bench_logits}[a.op](a)
     for r in rows:
         if "tflops" in r:
             r[f"frac_of_{pk['src']}_gemm_peak"] = round(r["tflops"] / pk["tflops"], 3)
