@@ -497,13 +497,13 @@ def bench_paged8(a) -> list[dict]:
         k, v = (torch.randn(B, Hk, L, hd, device="cuda").bfloat16() for _ in range(2))
         q = torch.randn(B, Hk * rep, 1, hd, device="cuda").bfloat16()
         qc = torch.randn(4, Hk * rep, 512, hd, device="cuda").bfloat16()
-        rows = 2 * B * Hk * L * hd
+        rows, last = 2 * B * Hk * L * hd, full - 1
         half = B * W // 2
         src = torch.arange(half, dtype=torch.int32, device="cuda")
         pools = [t.unsqueeze(0) for t in (kp, vp, ks, vs)]
         for name, nbytes, flops, fn in (
                 ("append_prompts", 3 * rows, 0, lambda: append_paged8(k, v, kp, vp, ks, vs, table, zero)),
-                ("append_token", 3 * rows // L, 0, lambda: append_paged8(k[:, :, :1], v[:, :, :1], kp, vp, ks, vs, table, full - 1)),
+                ("append_token", 3 * rows // L, 0, lambda: append_paged8(k[:, :, :1], v[:, :, :1], kp, vp, ks, vs, table, last)),
                 ("attend_token", rows, 4 * B * L * Hk * rep * hd, lambda: attend_paged8(q, kp, vp, ks, vs, table, full)),
                 ("attend_chunk512", 0, 4 * 4 * 512 * (L - 255) * Hk * rep * hd,
                  lambda: attend_paged8(qc, kp, vp, ks, vs, table[:4].contiguous(), full[:4].contiguous())),
