@@ -7,14 +7,17 @@
 // both products take it from shared memory (S^T = K Q^T: keys as M, rows as N; O^T = V^T P^T: dims as M).  The other
 // operand keeps its precision as a sum of two e4m3 numbers: q = 2^e (q_hi + q_lo) holds every bit of a bf16 query whose
 // elements lie within 2^10 of the row's largest (below that, 2^-19 of the largest), p likewise to 8 bits; both parts are
-// columns of one product (N = 2 x rows: the tile is read once for both) and are added when they are read.  Page scales stay outside: k_scale multiplies the thread's (key's) scores, the
-// v scales of a tile enter as p * v_scale / max(v_scale) and the maximum as a factor of the folded output.
+// columns of one product (N = 2 x rows: the tile is read once for both) and are added when they are read.  p_lo is held
+// times 32 (p_lo <= p_hi / 16), so that a weight keeps its 8 bits down to 2^-13 of its reference and a step of 2^-22 below.
+// The reference is the row's running maximum, or near the tile's own where that lies more than 2^4 lower: behind one key far
+// above all others the tiles without it lose nothing.  Page scales stay outside: k_scale multiplies the thread's (key's)
+// scores, the v scales of a tile enter as p * v_scale / max(v_scale) and the maximum as a factor of the folded output.
 //
 // Work: the tiles of all (sequence, KV head) items form one line that the CTAs split evenly (two CTAs per SM, as many as
 // there are tiles at most), so ragged lengths balance and a long single sequence fills the GPU.  An item inside one CTA
 // is finished there; one cut by a border leaves (maximum, sum, output) partials that the combine kernel merges in
 // the order of the keys, so results do not depend on timing.
-// Measured (B200, 8 query heads per KV head): 64 sequences x 4096 rows, 4 KV heads of 128, pages of 128: 54.6 us; its bytes
+// Measured (B200, 8 query heads per KV head): 64 sequences x 4096 rows, 4 KV heads of 128, pages of 128: 56.7 us; its bytes
 // alone take 41 us.  Time grows by 7.0 TB/s with the rows over about 20 us (fill, item changes, merge).  K and V in one
 // ring: 57 us; a second softmax group taking every other tile: 65 us.
 // Warps 0-3: softmax (thread = key) and output (thread = head-dim column); 4: TMA producer, page ids read two tiles and
@@ -35,6 +38,8 @@ constexpr int MAXR = 16;       // query rows of an item at most
 constexpr int NTHREADS = 192;
 constexpr int kMaxBlocksPerTile = 16;  // pages of 8 rows
 constexpr float kPOne = 256.f;         // probabilities are held times 2^8 (e4m3 reaches 448)
+constexpr float kPLow = 32.f;          // and what the high part leaves (8 at most) times 2^5
+constexpr float kFar = 4.f;            // log2 distance from the running maximum to a tile's that is left in the probabilities
 
 __device__ int g_error = 0;
 
@@ -395,7 +400,9 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       float m[NR], lpart[NR], acc[NR], alpha[NR], qf[NR];
       int lim[CAUSAL ? NR : 1];
       float vfac = 0.f;  // of the tile that is folded next, with alpha where its maximum grew
-      bool rescale = false;
+      bool rescale = false, far = false;
+      uint32_t down[NR / 4];  // log2 that its reference lies below the running maximum, a byte per row; where far
+      auto shift = [](const uint32_t* d, int h) { return (int)((d[h / 4] >> (h % 4 * 8)) & 0xff); };
       int nan_at = 0x7fffffff;  // first key whose value in this thread's column is NaN (tiles that a row sees partly)
       compute_sync();           // row factors of this item are written
 #pragma unroll
@@ -425,7 +432,8 @@ __global__ void __launch_bounds__(NTHREADS, 2)
 #pragma unroll
         for (int h = 0; h < NR; ++h) {
           if (rescale) acc[h] *= alpha[h];
-          acc[h] = fmaf(__uint_as_float(r[h]) + __uint_as_float(r[NP + h]), vfac, acc[h]);
+          const float o = fmaf(__uint_as_float(r[NP + h]), 1.f / kPLow, __uint_as_float(r[h]));
+          acc[h] = fmaf(o, far ? vfac * p8::pow2(-shift(down, h)) : vfac, acc[h]);
         }
       };
       const Walk cur = w;
@@ -493,6 +501,18 @@ __global__ void __launch_bounds__(NTHREADS, 2)
             m[h] = mn;
           }
         }
+        bool far_now = false;  // the same in all threads, too
+#pragma unroll
+        for (int h = 0; h < NR; ++h) far_now = far_now || m[h] - mx[h] > kFar;
+        uint32_t down_now[NR / 4];
+        if (far_now) {
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const float gap = m[h] - mx[h];  // no key of the tile seen: infinite, no weight either; none so far: NaN
+            const uint32_t d = gap > kFar ? (uint32_t)fminf(gap, 126.f) : 0;
+            down_now[h / 4] = h % 4 ? down_now[h / 4] | d << (h % 4 * 8) : d;
+          }
+        }
         uint8_t* pb = sm + C::P_OFF + sb * NB * TK;
         const int prow = tid & 15, pcol = tid >> 4;
 #pragma unroll
@@ -506,11 +526,12 @@ __global__ void __launch_bounds__(NTHREADS, 2)
           }
           lpart[h] += e0;
           lpart[h + 1] += e1;
+          if (far_now) e0 *= p8::pow2(shift(down_now, h)), e1 *= p8::pow2(shift(down_now, h + 1));
           // p to 8 bits: the nearest e4m3 number and the nearest one to what is left (f16 between: 11 bits)
           const __half2 p16 = __floats2half2_rn(e0 * vr, e1 * vr);
           const __nv_fp8x2_storage_t hi = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&p16), __NV_SATFINITE, __NV_E4M3);
           const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3);
-          const __half2 rest = __hsub2(p16, *reinterpret_cast<const __half2*>(&back));
+          const __half2 rest = __hmul2(__hsub2(p16, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(kPLow));
           const __nv_fp8x2_storage_t lo2 = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&rest), __NV_SATFINITE, __NV_E4M3);
           uint8_t* d0 = pb + swz<128>(h, pcol) + prow;
           uint8_t* d1 = pb + swz<128>(h + 1, pcol) + prow;
@@ -544,6 +565,11 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         if (grown) {
 #pragma unroll
           for (int h = 0; h < NR; ++h) alpha[h] = alpha_now[h];
+        }
+        far = far_now;
+        if (far_now) {
+#pragma unroll
+          for (int k = 0; k < NR / 4; ++k) down[k] = down_now[k];
         }
         vfac = tv.x * (1.f / kPOne);
       }

@@ -144,8 +144,8 @@ def attend_paged8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k
     ``q_lens[b]`` (all ``S`` without) stands at position ``lens[b] + len_add - q_lens[b] + i`` and sees the rows up to
     its own.  Rows past ``q_lens`` and rows that see no key are zero; pages outside the pool read as zeros.
     Repeated calls agree bit for bit; a sequence's rounding may change with the lengths of the others, which decide
-    where its keys are cut into parts.  Value pages are weighed by their scale against the largest beside them: scales
-    more than 2^10 apart within 128 keys (few query rows) leave the smaller page's weights fewer than 8 bits.
+    where its keys are cut into parts.  Weights are held in 8 bits (few query rows) down to 2^-13 of the largest among
+    the 128 keys of a tile, in a step of 2^-22 of it below; a value page's scale below the tile's largest counts there.
     Inference only (no gradient)."""
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention over the 8-bit cache has no backward: call it under torch.no_grad()")
