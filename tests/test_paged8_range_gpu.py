@@ -96,3 +96,13 @@ def test_small_weights_behind_a_sink_few_rows(B, Hk, rep, hd, bs, n, S, gap, sin
     c = _case(B, Hk, rep, hd, bs, n, S, gap, sinks)
     got = attend_paged8(*c, scale=1.0)
     _agree(got, *_attend64(*c, 1.0, few=True))
+
+
+@pytest.mark.parametrize("gap", [9.0, 13.0, 15.0, 16.0])
+@pytest.mark.parametrize("B,Hk,rep,hd,bs,n,S", [(8, 2, 8, 128, 64, 8191, 33), (24, 2, 5, 64, 16, 3000, 60)])
+def test_small_weights_behind_a_sink_many_rows(B, Hk, rep, hd, bs, n, S, gap):
+    from verl_omni_b200.ops.paged8 import attend_paged8
+
+    c = _case(B, Hk, rep, hd, bs, n, S, gap, 1)
+    got = attend_paged8(*c, scale=1.0)
+    _agree(got, *_attend64(*c, 1.0, few=False))

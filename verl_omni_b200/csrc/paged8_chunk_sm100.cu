@@ -6,12 +6,13 @@
 // every e4m3 number is an f16 number, and the page scales, powers of two, enter as code * scale / (largest scale of the
 // CTA's key range) (exact down to 2^-24 of it).  Probabilities are f16 too (11 bits), kept in tensor memory over the scores
 // they come from; queries are brought to [2^7, 2^9) by a power of two per row, exact for bf16.  Running maximum with a
-// lazy rescale of the output (only when it grows by more than 2^8), fp32 sums.
+// lazy rescale of the output (only when it grows by more than 2^8), fp32 sums.  Probabilities are held times 2^7, up to 2^15
+// with the laziness: they keep 11 bits down to 2^-21 of the maximum and 8 down to 2^-24, below in steps of 2^-31.
 // Work: as in the kernel for few rows, the 128-key tiles of all (sequence, KV head, 256 rows) items form one line split
 // evenly over one CTA per SM; causal items are as long as their last row's reach; cut items are merged in key order.
 // Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-11 and 12-14: K and V pages -> f16 tiles in
 // shared memory (the codes come by TMA, a tile ahead); 15: tensor-memory allocation, MMA issue.
-// Measured (B200): 4 x 512 tokens on 8000 rows, 32 query and 4 KV heads of 128: 367 us, 707 TFLOP/s.  What bounds it is the
+// Measured (B200): 4 x 512 tokens on 8000 rows, 32 query and 4 KV heads of 128: 370 us, 702 TFLOP/s.  What bounds it is the
 // chain of a tile (scores, softmax, second product): leaving out the stores of the conversion, the exponentials or half of
 // either product gained 3 to 9 % each.  64-key tiles with the scores a tile ahead: 513 us.
 // The loops are kept short (few unrolled copies): five roles run at once, and with everything unrolled the warps mostly
@@ -38,6 +39,7 @@ constexpr int KST = 1, VST = 2;       // f16 K and V tiles: a K tile is free for
 // the MMA warp, and that two tiles behind the loaders: a buffer is neither refilled nor its phase passed over before then.
 constexpr int kSegs = 6;
 constexpr float kLazy = 8.f;          // log2 growth of the maximum that is left in the probabilities
+constexpr float kUp = 7.f;            // and log2 of what one at the maximum is held as: f16 reaches 2^16
 
 __device__ int g_error = 0;
 
@@ -607,7 +609,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             st32(O_t + c * 32, o);
           }
         }
-        const float nmb = m == -INFINITY ? 0.f : -m;
+        const float nmb = m == -INFINITY ? 0.f : kUp - m;
         float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll 1
         for (int g = 0; g < 2; ++g) {  // probabilities of 64 keys, f16 pairs over scores that have been read

@@ -144,8 +144,9 @@ def attend_paged8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k
     ``q_lens[b]`` (all ``S`` without) stands at position ``lens[b] + len_add - q_lens[b] + i`` and sees the rows up to
     its own.  Rows past ``q_lens`` and rows that see no key are zero; pages outside the pool read as zeros.
     Repeated calls agree bit for bit; a sequence's rounding may change with the lengths of the others, which decide
-    where its keys are cut into parts.  Weights are held in 8 bits (few query rows) down to 2^-13 of the largest among
-    the 128 keys of a tile, in a step of 2^-22 of it below; a value page's scale below the tile's largest counts there.
+    where its keys are cut into parts.  Weights keep 8 bits down to 2^-9 of the largest among the 128 keys of a tile (up
+    to 16 query rows: tokens times heads of a group) or 2^-24 of the row's largest so far (more), below in steps of
+    2^-18 and 2^-31 of it; a value page's scale below the largest beside it counts as a smaller weight there.
     Inference only (no gradient)."""
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention over the 8-bit cache has no backward: call it under torch.no_grad()")
