@@ -106,3 +106,28 @@ def test_small_weights_behind_a_sink_many_rows(B, Hk, rep, hd, bs, n, S, gap):
     c = _case(B, Hk, rep, hd, bs, n, S, gap, 1)
     got = attend_paged8(*c, scale=1.0)
     _agree(got, *_attend64(*c, 1.0, few=False))
+
+
+@pytest.mark.parametrize("rep,S", [(8, 1), (2, 1), (16, 1), (5, 3)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_queries_with_one_large_element(hd, rep, S):
+    """Eight elements 2^14 below the largest, which meets zeros in every key: the scores come from the small ones.  Queries are two
+    e4m3 numbers relative to a power of two 2^e with max |q| <= 448 * 2^e, the low one times 16: a rounding of 2^-14 * 2^e at most
+    per element, so of that times sum |k| * scale per score, and of twice the largest of it times sum p |v| in the output."""
+    from verl_omni_b200.ops.paged8 import attend_paged8
+
+    torch.manual_seed(0)
+    B, Hk, bs, n = 4, 2, 16, 500
+    scale = 4 * 2.0 ** 14 / 8 ** 0.5  # scores with a spread of about 4
+    q = torch.zeros(B, Hk * rep, S, hd, device="cuda")
+    q[..., 3:11] = torch.randn(B, Hk * rep, S, 8, device="cuda") * 2.0 ** -14
+    q[..., 0] = 1.0
+    k = torch.randn(140, Hk, bs, hd, device="cuda")
+    k[..., 0] = 0.0
+    (kp, ks), (vp, vs) = _codes(k), _codes(torch.randn(140, Hk, bs, hd, device="cuda"))
+    c = (q.bfloat16(), kp, vp, ks, vs, _table(B, -(-n // bs), 140), torch.full((B,), n, dtype=torch.int32, device="cuda"))
+    want, tol = _attend64(*c, scale, few=True)
+    keys = (_values(kp.view(torch.uint8)) * ks.double()[..., None, None])[..., 3:11].abs().sum(-1).amax()
+    weighed, _ = _attend64(*c[:2], vp.view(torch.uint8).bitwise_and(0x7F).view(E4M3), *c[3:], scale, few=True)  # sum p |v|
+    tol = tol + 2 * 2.0 ** -14 * 2.0 ** -8 * float(keys) * scale * weighed
+    _agree(attend_paged8(*c, scale=scale), want, tol)

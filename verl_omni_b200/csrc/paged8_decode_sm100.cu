@@ -6,12 +6,13 @@
 // The e4m3 codes go from global memory to the tensor core as they are: a 128-key tile of K and V is staged by TMA, and
 // both products take it from shared memory (S^T = K Q^T: keys as M, rows as N; O^T = V^T P^T: dims as M).  The other
 // operand keeps its precision as a sum of two e4m3 numbers: q = 2^e (q_hi + q_lo) holds every bit of a bf16 query whose
-// elements lie within 2^10 of the row's largest (below that, 2^-19 of the largest), p likewise to 8 bits; both parts are
-// columns of one product (N = 2 x rows: the tile is read once for both) and are added when they are read.  p_lo is held
-// times 32 (p_lo <= p_hi / 16), so that a weight keeps its 8 bits down to 2^-13 of its reference and a step of 2^-22 below.
-// The reference is the row's running maximum, or near the tile's own where that lies more than 2^4 lower: behind one key far
-// above all others the tiles without it lose nothing.  Page scales stay outside: k_scale multiplies the thread's (key's)
-// scores, the v scales of a tile enter as p * v_scale / max(v_scale) and the maximum as a factor of the folded output.
+// elements lie within 2^13 of the row's largest (a rounding of 2^-21 of the largest below), p likewise to 8 bits; both parts
+// are columns of one product (N = 2 x rows: the tile is read once for both) and are added when they are read.  The low part
+// is at most 1/16 of the high one: q_lo is held times 16 and p_lo (p <= 256) times 32, so that a weight keeps its 8 bits down
+// to 2^-13 of its reference, with steps of 2^-22 below.  The reference is the row's running maximum, or near the tile's own
+// where that lies more than 2^4 lower: behind one key far above all others the tiles without it lose nothing.  Page scales stay
+// outside: k_scale multiplies the thread's (key's) scores, the v scales of a tile enter as p * v_scale / max(v_scale) and the
+// maximum as a factor of the folded output.
 //
 // Work: the tiles of all (sequence, KV head) items form one line that the CTAs split evenly (two CTAs per SM, as many as
 // there are tiles at most), so ragged lengths balance and a long single sequence fills the GPU.  An item inside one CTA
@@ -37,6 +38,7 @@ constexpr int TK = 128;        // keys per tile
 constexpr int MAXR = 16;       // query rows of an item at most
 constexpr int NTHREADS = 192;
 constexpr int kMaxBlocksPerTile = 16;  // pages of 8 rows
+constexpr float kQLow = 16.f;          // what the high part of a query leaves (16 at most) is held times 2^4
 constexpr float kPOne = 256.f;         // probabilities are held times 2^8 (e4m3 reaches 448)
 constexpr float kPLow = 32.f;          // and what the high part leaves (8 at most) times 2^5
 constexpr float kFar = 4.f;            // log2 distance from the running maximum to a tile's that is left in the probabilities
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         const uint2 hi = p8::pack_e4m3x8(f);
         p8::unpack_e4m3x8(hi, lo8);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) lo8[i] = f[i] - lo8[i];
+        for (int i = 0; i < 8; ++i) lo8[i] = (f[i] - lo8[i]) * kQLow;
         uint8_t* q = sm + C::Q_OFF + swz<HD>(r, c >> 1) + (c & 1) * 8;
         *reinterpret_cast<uint2*>(q) = hi;
         *reinterpret_cast<uint2*>(q + NP * HD) = p8::pack_e4m3x8(lo8);
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         mbar_arrive(&s_empty[sb]);
         float s[NR];
 #pragma unroll
-        for (int h = 0; h < NR; ++h) s[h] = (__uint_as_float(r[h]) + __uint_as_float(r[NP + h])) * (ksc * qf[h]);
+        for (int h = 0; h < NR; ++h) s[h] = fmaf(__uint_as_float(r[NP + h]), 1.f / kQLow, __uint_as_float(r[h])) * (ksc * qf[h]);
         bool there = true;
         if (!full) {
           there = t < cur.len && ksc != 0.f;
