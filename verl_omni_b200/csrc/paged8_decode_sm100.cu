@@ -548,6 +548,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
 #pragma unroll
             for (int c = 0; c < HD / 16; ++c) reinterpret_cast<uint4*>(vt + tid * HD)[c] = make_uint4(0, 0, 0, 0);
           }
+          if (CAUSAL && tv.y != 0.f) compute_sync();  // zeroed before they are looked through below
           if (CAUSAL && tid < HD) {
             // some row may see only part of this tile: a NaN value must not reach it through 0 * NaN
             for (int k = 0; k < min(TK, cur.len - t0); ++k) {
