@@ -255,6 +255,14 @@ bool rows_ok(const torch::Tensor& t) {
          reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
 
+// the tensor itself, or a copy that satisfies rows_ok (a contiguous one may still start off a 16-byte boundary; dimensions of
+// one element keep their strides, which are not used)
+torch::Tensor vector_rows(torch::Tensor t) {
+  if (rows_ok(t)) return t;
+  t = t.contiguous();
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 void check_i32(const torch::Tensor& t, const char* name, int64_t n, const torch::Tensor& like) {
   TORCH_CHECK_VALUE(t.scalar_type() == torch::kInt32 && t.dim() == 1 && t.size(0) == n && t.is_contiguous() &&
                         t.device() == like.device(),
@@ -304,8 +312,8 @@ void paged8_append(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Te
   TORCH_CHECK_VALUE(S < (1 << 30) && Hk <= 65535 && offset >= 0 && offset < (1 << 30), "tokens, kv_heads or offset out of range");
   if (B == 0 || S == 0) return;
   c10::cuda::CUDAGuard g(k.device());
-  if (!rows_ok(k)) k = k.contiguous();
-  if (!rows_ok(v)) v = v.contiguous();
+  k = vector_rows(k);
+  v = vector_rows(v);
   const int block = (int)kp.size(2);
   const int touched = (int)((S + block - 2) / block + 1);
   TORCH_CHECK_VALUE(B * touched < (1ll << 31), "batch x pages out of range");
@@ -380,7 +388,7 @@ torch::Tensor paged8_attend(torch::Tensor q, torch::Tensor kp, torch::Tensor vp,
   c10::cuda::CUDAGuard g(q.device());
   auto out = torch::empty({B, S, Hq, hd}, q.options());
   if (out.numel() == 0) return out;
-  if (!rows_ok(q)) q = q.contiguous();
+  q = vector_rows(q);
   TORCH_CHECK_VALUE(B * S * Hq < (1ll << 31), "batch x tokens x heads out of range");
   p8::AttendArgs a{bf_of(q), q.stride(0), q.stride(1), q.stride(2), bytes_of(kp), bytes_of(vp), ks.data_ptr<float>(),
                    vs.data_ptr<float>(), table.data_ptr<int>(), lens.data_ptr<int>(), ql,
