@@ -24,3 +24,16 @@ def pytest_collection_modifyitems(config, items):
             item.add_marker(pytest.mark.skip(reason="no CUDA GPU"))
         if "multigpu" in item.keywords and n_gpu < 2:
             item.add_marker(pytest.mark.skip(reason="needs 2+ GPUs"))
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(request):
+    """After a GPU test of the 8-bit paged cache: no bounded wait inside its kernels ran out."""
+    yield
+    if "gpu" in request.keywords and request.module.__name__.startswith("test_paged8"):
+        import torch
+
+        from verl_omni_b200.ops import paged8
+
+        if torch.cuda.is_available():
+            paged8.raise_on_timeout("cuda")

@@ -147,13 +147,27 @@ def attend_paged8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k
     where its keys are cut into parts.  Weights keep 8 bits down to 2^-9 of the largest among the 128 keys of a tile (up
     to 16 query rows: tokens times heads of a group) or 2^-24 of the row's largest so far (more), below in steps of
     2^-18 and 2^-31 of it; a value page's scale below the largest beside it counts as a smaller weight there.
-    Inference only (no gradient)."""
+    Inference only (no gradient).  Waits inside the kernels are bounded: :func:`raise_on_timeout` tells whether one ran out."""
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention over the 8-bit cache has no backward: call it under torch.no_grad()")
     if not q.is_cuda:
         return attend_paged8_reference(q, k_pool, v_pool, k_scale, v_scale, block_table, lens, q_lens, scale, len_add)
     return _ext().paged8_attend(q, k_pool, v_pool, k_scale, v_scale, block_table, lens, q_lens,
                                 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale, len_add)
+
+
+def raise_on_timeout(device) -> None:
+    """Raises a RuntimeError if a bounded wait of the attention kernels ran out on ``device`` since the last call: what they
+    wrote is then not an attention output.  Waits for the current stream; for the end of a rollout or a step, where results
+    are read anyway."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        return
+    with torch.cuda.device(device):
+        torch.cuda.current_stream().synchronize()
+        code = _ext().paged8_error(True)
+    if code:
+        raise RuntimeError(f"8-bit attention: a wait inside the kernel ran out (code {code}), its outputs are invalid")
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Union[torch.Tensor, Sequence[int]],

@@ -18,7 +18,7 @@ import torch
 from verl_omni_b200.models.moe_llm import MoELLM
 from verl_omni_b200.ops.decode import KVCache, PagedKVCache, sample_tokens
 from verl_omni_b200.ops.logits import process_logits
-from verl_omni_b200.ops.paged8 import Paged8View, PagedKVCache8
+from verl_omni_b200.ops.paged8 import Paged8View, PagedKVCache8, raise_on_timeout
 from verl_omni_b200.utils.dataproto import DataProto
 
 
@@ -227,6 +227,8 @@ class LLMRolloutEngine:
                 else:
                     logits = self.module(nxt[:, None], caches=caches, pos0=P + t)[:, -1]
         lp = torch.stack(out_lp, 1)
+        if self.kv8:
+            raise_on_timeout(dev)
         if tp is not None:
             own = slice(tp.rank * B_own, (tp.rank + 1) * B_own)
             ids, lp = ids[own], lp[own]
