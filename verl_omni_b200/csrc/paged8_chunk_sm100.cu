@@ -297,16 +297,19 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       off_n = t % a.block;
     };
     auto scale_of_page = [&](int kh, int id) { return id >= 0 && id < a.pages ? __ldg(sc + (int64_t)id * a.Hk + kh) : 0.f; };
-    // starts its copies (the role's first warp, lane = page) and reads its scale; 0: no such page
-    auto start_tile = [&]() {
+    int started = 0;  // tiles whose copies were started
+    // starts its copies (the role's first warp, lane = page) and reads its scale; 0: no such page.  Nothing is started where
+    // the tile before was given up (landed false): its copies may still be on their way to the same place
+    auto start_tile = [&](bool landed) {
       const int base = id_n >= 0 && id_n < a.pages ? (id_n * a.Hk + kh_n) * a.block + off_n : -1;
-      if (lw == 0) {
+      if (lw == 0 && __all_sync(0xffffffffu, landed)) {
         const int row = __shfl_sync(0xffffffffu, base, (lane * blk >> 3) & 15);
         const bool load = lane < nblk && row >= 0;
         const unsigned n = __popc(__ballot_sync(0xffffffffu, load));
         if (lane == 0) mbar_expect_tx(raw_full, n * blk * HD);
         __syncwarp();
         if (load) tma_load_2d(smem_u32(codes) + lane * blk * HD, map, raw_full, 0, row);
+        ++started;
       }
       return scale_of_page(kh_n, id_n);
     };
@@ -370,7 +373,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     float inv_ref = 1.f, s0 = 0.f;
     if (ntot > 0) {
       fetch(w);
-      s0 = start_tile();
+      s0 = start_tile(true);
     }
     for (int i = 0; i < ntot; ++i) {
       if (left == 0) {
@@ -402,16 +405,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if (--left == 0) next_item(w, p);
       else ++w.tile;
       if (i + 1 < ntot) fetch(w);
-      mbar_wait(raw_full, i & 1, abort_flag, &g_error, V ? 25 : 24);
+      const bool landed = mbar_wait(raw_full, i & 1, abort_flag, &g_error, V ? 25 : 24);
       mbar_wait(&empty[i % ST], ((i / ST) & 1) ^ 1, abort_flag, &g_error, V ? 23 : 22);
       // V: where some row sees only part of the tile, a NaN value must not reach it through 0 * NaN
       convert(tiles + (i % ST) * C::TILE, n, s0 * inv_ref, V && t0 + TK > common ? nan_at + buf * HD : nullptr, t0);
       mbar_arrive(&full[i % ST]);
       loader_sync<V>();  // every loader has read the codes: their place is refilled
-      if (i + 1 < ntot) s0 = start_tile();
+      if (i + 1 < ntot) s0 = start_tile(landed);
       if (V && left == 0) mbar_arrive(&nan_full[buf]);
     }
-    if (*abort_flag && lt == 0 && ntot > 0) mbar_drain(raw_full, (ntot - 1) & 1);  // copies in flight land before the CTA leaves
+    if (*abort_flag && lt == 0 && started > 0) mbar_drain(raw_full, (started - 1) & 1);  // copies in flight land before the CTA leaves
   };
   if (warp >= 8 && warp < 12) {
     loader(std::false_type{});

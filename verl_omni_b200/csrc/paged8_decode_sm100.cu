@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     if (ntot > 1) fetch(f1);
     float2 s0 = scales(f0);
     if (ntot > 0) issue(f0, &mk, &k_full[0], base);
-    int issued = 0;
+    int issued = 0, k_issued = min(ntot, 1);
     for (int i = 0; i < ntot; ++i) {
       Pre f2{-2, 0, 0};
       if (i + 2 < ntot) fetch(f2);
@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         if (lane == 0) ok = mbar_wait(&k_empty[st], (((i + 1) / SK) & 1) ^ 1, abort_flag, &g_error, 1);
         if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
         issue(f1, &mk, &k_full[st], base + st * C::KV);
+        k_issued = i + 2;
       }
       const int st = i % SV;
       bool ok = true;
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     }
     if (lane == 0 && *abort_flag) {  // the copies in flight land before the CTA leaves
       for (int i = max(0, issued - SV); i < issued; ++i) mbar_drain(&v_full[i % SV], (i / SV) & 1);
-      for (int i = max(0, issued + 1 - SK); i < min(ntot, issued + 1); ++i) mbar_drain(&k_full[i % SK], (i / SK) & 1);
+      for (int i = max(0, k_issued - SK); i < k_issued; ++i) mbar_drain(&k_full[i % SK], (i / SK) & 1);
     }
     __syncwarp();
   } else if (warp == 5) {
