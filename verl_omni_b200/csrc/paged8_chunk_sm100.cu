@@ -296,9 +296,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       id_n = t < x.len ? __ldg(a.table + (int64_t)x.b * a.width + t / a.block) : -1;
       off_n = t % a.block;
     };
-    auto scale_of_page = [&](int kh, int id) { return id >= 0 && id < a.pages ? __ldg(sc + (int64_t)id * a.Hk + kh) : 0.f; };
+    constexpr float kNoPage = -1.f;
+    auto scale_of_page = [&](int kh, int id) { return id >= 0 && id < a.pages ? __ldg(sc + (int64_t)id * a.Hk + kh) : kNoPage; };
     int started = 0;  // tiles whose copies were started
-    // starts its copies (the role's first warp, lane = page) and reads its scale; 0: no such page.  Nothing is started where
+    // starts its copies (the role's first warp, lane = page) and reads its scale.  Nothing is started where
     // the tile before was given up (landed false): its copies may still be on their way to the same place
     auto start_tile = [&](bool landed) {
       const int base = id_n >= 0 && id_n < a.pages ? (id_n * a.Hk + kh_n) * a.block + off_n : -1;
@@ -313,8 +314,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       return scale_of_page(kh_n, id_n);
     };
-    // code * scale / ref in f16, 64-column groups of swizzled 128-byte rows; rows from n on and rows without a page are
-    // zero.  The two halves of a piece are written in the other order in the odd groups, so that a row's eight lanes
+    // code * scale / ref in f16, 64-column groups of swizzled 128-byte rows; rows from n on and rows without a page (a
+    // negative factor; one that is zero in f16 still leaves NaN) are zero.  The two halves of a piece are written in the other order in the odd groups, so that a row's eight lanes
     // hit different banks.  nan: first keys with a NaN per column are noted and the value left out.
     auto convert = [&](uint8_t* dst, int n, float factor, int* nan, int t0) {
       const __half2 mine_f = __float2half2_rn(factor);
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           const int r = (b0 + i) * RP + r_in;
           fs[i] = __shfl_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&mine_f), (r >> 3) & 15);
           d[i] = *reinterpret_cast<const uint4*>(codes + min(r, TK - 1) * HD + c * 16);
-          if (r >= min(n, TK) || fs[i] == 0) d[i] = make_uint4(0, 0, 0, 0);
+          if (r >= min(n, TK) || (fs[i] & 0x8000u)) d[i] = make_uint4(0, 0, 0, 0);
         }
         if (V && nan != nullptr) {
 #pragma unroll
