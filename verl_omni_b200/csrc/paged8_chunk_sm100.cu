@@ -3,11 +3,12 @@
 //
 // Here the bound is arithmetic: the exponentials and the two products of rows x keys.  Query rows (token, head of the KV
 // group) are the M of both products, 256 rows a CTA in two tiles of 128; keys and values become f16 once per 256 rows:
-// every e4m3 number is an f16 number, and the page scales, powers of two, enter as code * scale / (largest scale of the
-// CTA's key range) (exact down to 2^-24 of it).  Probabilities are f16 too (11 bits), kept in tensor memory over the scores
-// they come from; queries are brought to [2^7, 2^9) by a power of two per row, exact for bf16.  Running maximum with a
-// lazy rescale of the output (only when it grows by more than 2^8), fp32 sums.  Probabilities are held times 2^7, up to 2^15
-// with the laziness: they keep 11 bits down to 2^-21 of the maximum and 8 down to 2^-24, below in steps of 2^-31.
+// every e4m3 number is an f16 number, and the page scales enter as code * scale / (largest scale of the CTA's key range)
+// (powers of two: exact down to 2^-24 of it; other scales to 11 bits).  Probabilities are f16 too (11 bits), kept in tensor
+// memory over the scores they come from; queries are brought to [2^7, 2^9) by a power of two per row, exact for bf16.
+// Running maximum with a lazy rescale of the output (only when it grows by more than 2^8), fp32 sums.  Probabilities are
+// held times 2^7, up to 2^15 with the laziness: they keep 11 bits down to 2^-21 of the maximum and 8 down to 2^-24, below in
+// steps of 2^-31.
 // Work: as in the kernel for few rows, the 128-key tiles of all (sequence, KV head, 256 rows) items form one line split
 // evenly over one CTA per SM; causal items are as long as their last row's reach; cut items are merged in key order.
 // Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-11 and 12-14: K and V pages -> f16 tiles in
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         loader_sync<V>();
         m = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], V ? 0.f : pm[3]));
         m = m > 0.f ? m : 1.f;
-        inv_ref = inv_pow2(m);
+        inv_ref = 1.f / m;
         common = max(1, w.len - w.nq + (int)((int64_t)w.rt * ROWS / a.rep) + 1);  // keys below: seen by every row that sees any
         // buffers seg % kSegs were last read by the softmax several items ago: this wait is past that
         mbar_wait(&empty[i % ST], ((i / ST) & 1) ^ 1, abort_flag, &g_error, V ? 26 : 21);

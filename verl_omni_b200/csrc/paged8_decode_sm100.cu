@@ -57,7 +57,7 @@ struct Cfg {
   static constexpr int Q_OFF = V_OFF + SV * KV;         // NB rows of HD bytes
   static constexpr int P_OFF = Q_OFF + NB * HD;         // two buffers of NB rows of TK bytes
   static constexpr int SC_OFF = P_OFF + 2 * NB * TK;    // per V tile: k and v scale of each page
-  static constexpr int TV_OFF = SC_OFF + SV * 2 * kMaxBlocksPerTile * 4;       // per V tile: largest v scale, whether a page is missing
+  static constexpr int TV_OFF = SC_OFF + SV * 2 * kMaxBlocksPerTile * 4;       // per V tile: largest v scale, whether a page is missing, 2^8 / the former
   static constexpr int RED_OFF = TV_OFF + SV * 16;                             // [2][4][MAXR] warp maxima
   static constexpr int QS_OFF = RED_OFF + 2 * 4 * MAXR * 4;                    // [2][MAXR] row factors
   static constexpr int BAR_OFF = QS_OFF + 2 * MAXR * 4;
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     auto in_pool = [&](const Pre& f) { return f.id >= 0 && f.id < a.pages; };
     auto scales = [&](const Pre& f) {
       const int64_t i = (int64_t)f.id * a.Hk + f.kh;
-      return in_pool(f) ? make_float2(__ldg(a.ks + i), __ldg(a.vs + i)) : make_float2(0.f, 0.f);
+      return in_pool(f) ? make_float2(__ldg(a.ks + i), __ldg(a.vs + i)) : make_float2(-1.f, 0.f);
     };
     // the copies of one tile into ring place st of `full`, lane = page
     auto issue = [&](const Pre& f, const CUtensorMap* m, uint64_t* full, uint32_t dst) {
@@ -254,13 +254,13 @@ __global__ void __launch_bounds__(NTHREADS, 2)
       if (lane == 0) ok = mbar_wait(&v_empty[st], ((i / SV) & 1) ^ 1, abort_flag, &g_error, 11);
       if (!__shfl_sync(0xffffffffu, ok ? 1 : 0, 0)) break;
       if (lane < nblk) {
-        scl[(st * 2) * kMaxBlocksPerTile + lane] = s0.x;  // 0: no such page, its rows read as zeros
+        scl[(st * 2) * kMaxBlocksPerTile + lane] = s0.x;  // negative: no such page, its rows read as zeros
         scl[(st * 2 + 1) * kMaxBlocksPerTile + lane] = s0.y;
       }
       (void)VO_DCHECK(in_pool(f0) || f0.id == -2);  // checked builds record a page id outside the pool
       const float vmax = warp_fmax(s0.y);  // 0 without a page
       const bool missing = __any_sync(0xffffffffu, lane < nblk && !in_pool(f0));
-      if (lane == 0) tile_v[st * 4] = vmax, tile_v[st * 4 + 1] = missing ? 1.f : 0.f;
+      if (lane == 0) *reinterpret_cast<float4*>(tile_v + st * 4) = make_float4(vmax, missing ? 1.f : 0.f, vmax > 0.f ? kPOne / vmax : 0.f, 0.f);
       __syncwarp();
       issue(f0, &mv, &v_full[st], base + C::V_OFF + st * C::KV);
       issued = i + 1;
@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         ld_nowait(trow + S_COL + sb * NB, r);
         const float ksc = scl[(st * 2) * kMaxBlocksPerTile + my_blk];
         float vsc = scl[(st * 2 + 1) * kMaxBlocksPerTile + my_blk];
-        const float2 tv = *reinterpret_cast<const float2*>(tile_v + st * 4);
+        const float4 tv = *reinterpret_cast<const float4*>(tile_v + st * 4);
         // a whole tile: every row sees all of its keys, all its pages exist
         const bool full = t0 + TK <= common && tv.y == 0.f;
         wait_ld();
@@ -464,12 +464,12 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         for (int h = 0; h < NR; ++h) s[h] = fmaf(__uint_as_float(r[NP + h]), 1.f / kQLow, __uint_as_float(r[h])) * (ksc * qf[h]);
         bool there = true;
         if (!full) {
-          there = t < cur.len && ksc != 0.f;
+          there = t < cur.len && !(ksc < 0.f);
           if (!there) vsc = 0.f;
 #pragma unroll
           for (int h = 0; h < NR; ++h) {
             const bool seen = CAUSAL ? t < lim[h] : t < lim[0];
-            s[h] = !seen ? -INFINITY : ksc == 0.f ? 0.f : s[h];
+            s[h] = !seen ? -INFINITY : ksc < 0.f ? 0.f : s[h];
           }
         }
         float4* rd = reinterpret_cast<float4*>(red + sb * 4 * MAXR);  // [warp][row]
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
           if (lane == 0) rd[warp * (MAXR / 4) + h / 4] = v;
         }
         compute_sync();
-        const float vr = tv.x > 0.f ? vsc * inv_pow2(tv.x) * kPOne : 0.f;
+        const float vr = vsc * tv.z;
         float mx[NR];
         bool grown = false;
 #pragma unroll

@@ -140,7 +140,9 @@ def attend_paged8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k
                   q_lens: Optional[torch.Tensor] = None, scale: Optional[float] = None, len_add: int = 0) -> torch.Tensor:
     """q ``[B, Hq, S, hd]`` (any strides) against the cached rows -> ``[B, S, Hq, hd]``.
 
-    ``lens[b] + len_add`` rows of sequence b are cached, the new tokens' among them; query token ``i`` of its
+    Pools ``[pages, Hk, block, hd]`` e4m3, positive scales ``[pages, Hk]`` fp32 (powers of two as :func:`append_paged8`
+    writes them; with others more than 16 query rows take codes times scale in 11 bits), ``block_table [B, max_pages]``,
+    ``lens [B]`` int32.  ``lens[b] + len_add`` rows of sequence b are cached, the new tokens' among them; query token ``i`` of its
     ``q_lens[b]`` (all ``S`` without) stands at position ``lens[b] + len_add - q_lens[b] + i`` and sees the rows up to
     its own.  Rows past ``q_lens`` and rows that see no key are zero; pages outside the pool read as zeros.
     Repeated calls agree bit for bit; a sequence's rounding may change with the lengths of the others, which decide
