@@ -124,7 +124,8 @@ class LLMRolloutEngine:
         ``repetition_penalty`` (tokens of prompt and response), ``presence_penalty`` / ``frequency_penalty`` (tokens of
         the response), ``logit_bias`` (fp32 ``[vocab]``) and ``allowed_tokens`` (called with the response ids so far
         ``[B, t]``, returns an int32 bitmask ``[B or 1, ceil(vocab / 32)]`` or None) shape the distribution that tokens are
-        drawn from; the returned log-probs are those of that distribution."""
+        drawn from; the returned log-probs are those of that distribution.  A row that has ended (``eos_id``) and is allowed
+        no token is filled up with ``eos_id`` at log-prob 0; one that has not ended is an error."""
         if kv_cache_dtype not in ("auto", "fp8_e4m3"):
             raise ValueError(f"unknown kv_cache_dtype {kv_cache_dtype!r}: auto or fp8_e4m3")
         shaped = (repetition_penalty != 1.0 or presence_penalty or frequency_penalty or logit_bias is not None
@@ -199,6 +200,7 @@ class LLMRolloutEngine:
             prompt_lens = said.clone()
         out_ids, out_lp = [], []
         done = torch.zeros(B, dtype=torch.bool, device=ids.device)
+        stuck = torch.zeros_like(done)  # rows that a mask left no token before their end
         mask = []
         step = None
         if self.max_new_tokens > 1 and tp is None and _graph_ok(self.module, caches, dev):
@@ -212,6 +214,11 @@ class LLMRolloutEngine:
             if self.temperature <= 0:
                 lp = torch.log_softmax(logits.float(), -1).gather(-1, nxt[:, None]).squeeze(-1)
             if history is not None:
+                if ok is not None:
+                    none = logits.amax(-1) == float("-inf")
+                    nxt = torch.where(none, 0 if self.eos_id is None else self.eos_id, nxt)
+                    lp = torch.where(none, 0.0, lp)
+                    stuck = stuck | (none & ~done)
                 history[:, P + t] = nxt
                 said += 1
             out_ids.append(nxt)
@@ -229,6 +236,8 @@ class LLMRolloutEngine:
         lp = torch.stack(out_lp, 1)
         if self.kv8:
             raise_on_timeout(dev)
+        if self.allowed_tokens is not None and bool(stuck.any()):
+            raise RuntimeError(f"allowed_tokens left no token to {int(stuck.sum())} of {B} rows before their end")
         if tp is not None:
             own = slice(tp.rank * B_own, (tp.rank + 1) * B_own)
             ids, lp = ids[own], lp[own]
