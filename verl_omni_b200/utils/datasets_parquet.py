@@ -194,7 +194,8 @@ class ParquetMLLMDPODataset:
 class ParquetOmniRLDataset:
     """Prompts for the omni GRPO / GSPO trainer.  Each batch is left-padded to ``max_prompt_length`` with
     ``pad_id`` (the thinker attends over the padding like any other prompt token, identically in the rollout
-    and the log-prob recompute); longer prompts keep their last ``max_prompt_length`` tokens.  Text prompts
+    and the log-prob recompute; ``prompt_pad`` holds each row's number of padding tokens, which penalties for repeated tokens
+    leave out); longer prompts keep their last ``max_prompt_length`` tokens.  Text prompts
     without ids are tokenized byte-level.  Feature arrays are stacked per batch (equal counts per row)."""
 
     def __init__(self, files, *, vocab: int, max_prompt_length: int, pad_id: int = 0, max_samples: int = -1,
@@ -213,11 +214,13 @@ class ParquetOmniRLDataset:
     def get_batch(self, ids: list[int], uid_prefix: str = "") -> DataProto:
         rows = [self.df.iloc[int(i) % len(self.df)].to_dict() for i in ids]
         out = torch.full((len(rows), self.L), self.pad, dtype=torch.long)
+        pad = torch.zeros(len(rows), dtype=torch.int32)
         for j, r in enumerate(rows):
             toks = list(r["prompt_ids"]) if r.get("prompt_ids") is not None else self.tok(_prompt_text(r["prompt"]))
             toks = [int(t) for t in toks][-self.L:]
             out[j, self.L - len(toks):] = torch.tensor(toks, dtype=torch.long)
-        t = {"input_ids": out}
+            pad[j] = self.L - len(toks)
+        t = {"input_ids": out, "prompt_pad": pad}
         for feat in ("audio_feats", "image_patches"):
             if feat in self.df.columns:
                 t[feat] = torch.stack([_tensor(r, feat) for r in rows])

@@ -39,6 +39,14 @@ def sample_next(logits: torch.Tensor, temperature: float, top_k: int, top_p: flo
     return torch.multinomial(probs.cpu(), 1, generator=generator).squeeze(-1).to(logits.device)
 
 
+def said_tokens(ids: torch.Tensor, pad: Optional[torch.Tensor]) -> torch.Tensor:
+    """Token ids ``[B, L]`` with the first ``pad[b]`` of each row out of the vocabulary (-1): no history for
+    :func:`~verl_omni_b200.ops.logits.process_logits`."""
+    if pad is None:
+        return ids
+    return ids.masked_fill(torch.arange(ids.shape[1], device=ids.device) < pad[:, None], -1)
+
+
 def _graph_ok(module: MoELLM, caches, dev) -> bool:
     """CUDA-graph decode applies to contiguous and 8-bit paged caches on a GPU.  With experts sharded over ranks the step holds
     collectives; those are captured only on request (``VO_DECODE_GRAPH_EP=1``), since every rank of the group
@@ -154,7 +162,10 @@ class LLMRolloutEngine:
     @torch.no_grad()
     def generate(self, batch: DataProto, seed: int = 0, group: int = 1) -> DataProto:
         """``group``: every ``group`` consecutive rows of the batch are the same prompt.  With the 8-bit cache it is
-        prefilled once and its pages are shared (the partly filled last one copied); otherwise it changes nothing."""
+        prefilled once and its pages are shared (the partly filled last one copied); otherwise it changes nothing.
+
+        ``prompt_pad`` (int32 ``[B]`` in the batch, optional): the padding tokens ahead of each prompt; the penalties do not
+        count them as said."""
         if self.pp is not None:
             return self._generate_pp(batch, seed)
         tp = self.tp
@@ -162,11 +173,13 @@ class LLMRolloutEngine:
         af, ip = batch.batch.get("audio_feats"), batch.batch.get("image_patches")
         af = af.to(ids.device) if af is not None else None
         ip = ip.to(ids.device) if ip is not None else None
+        pad = batch.batch.get("prompt_pad") if self.shaping is not None else None
+        pad = pad.to(ids.device) if pad is not None else None
         B_own = ids.shape[0]
         if tp is not None:
             # the group's prompts in group-rank order; every rank decodes all of them (same seed on every rank,
             # identical logits after the all-reduces, so the same draws) and keeps its own rows at the end
-            ids, af, ip = (self._gather(t, tp) if t is not None else None for t in (ids, af, ip))
+            ids, af, ip, pad = (self._gather(t, tp) if t is not None else None for t in (ids, af, ip, pad))
         B, P = ids.shape
         dev = ids.device
         g = torch.Generator(device=dev).manual_seed(int(seed))  # sampling stays on the device
@@ -195,7 +208,7 @@ class LLMRolloutEngine:
         history = None
         if self.shaping is not None:
             # prompt, then the tokens as they are drawn; the lengths in force are on the device
-            history = torch.cat([ids, ids.new_zeros(B, self.max_new_tokens)], 1)
+            history = torch.cat([said_tokens(ids, pad), ids.new_zeros(B, self.max_new_tokens)], 1)
             said = torch.full((B,), P, dtype=torch.int32, device=dev)
             prompt_lens = said.clone()
         out_ids, out_lp = [], []
@@ -283,7 +296,7 @@ class LLMRolloutEngine:
         out = DataProto({"prompts": ids, "responses": resp, "rollout_log_probs": lp,
                          "response_mask": torch.stack(mask, 1).float(),
                          "input_ids": torch.cat([ids, resp], 1)}, dict(batch.non_tensor_batch))
-        for k in ("audio_feats", "image_patches"):
+        for k in ("audio_feats", "image_patches", "prompt_pad"):
             if k in batch.batch:
                 out.batch[k] = batch.batch[k]
         return out
