@@ -379,18 +379,27 @@ class MoELLM(nn.Module):
 
     def forward(self, ids, positions=None, caches=None, pos0: int = 0, audio_feats=None, image_patches=None,
                 return_hidden: bool = False, targets: Optional[torch.Tensor] = None, temperature: float = 1.0,
-                pos_t: Optional[torch.Tensor] = None, tp_decode=None):
+                pos_t: Optional[torch.Tensor] = None, tp_decode=None, shaping: Optional[dict] = None):
         """Logits [B, S, V] (fp32); ``return_hidden``: the final hidden states; ``targets`` [B, S] (next-token
         ids per position): log p(target) [B, S] through the chunked vocabulary kernel, with no logits tensor
-        (under tensor parallelism each rank scores its own tokens and the log-probs are gathered).
+        (under tensor parallelism each rank scores its own tokens and the log-probs are gathered); with ``shaping``
+        (``history``, ``prompt_len``, penalties and bias of
+        :func:`~verl_omni_b200.ops.vocab_logprob.shaped_token_logprobs`) those of the response under the distribution that a
+        rollout with the same options draws from, 0 over the prompt.
 
         ``pos_t`` (int64 ``[1]`` on the device): a one-token decode step at that position against contiguous
         caches, with the RoPE rows and the KV write position taken on the device (``rope`` must already
         cover the position: the caller sizes the table before the step is captured)."""
-        from verl_omni_b200.ops.vocab_logprob import token_logprobs_from_hidden
+        from verl_omni_b200.ops.vocab_logprob import shaped_token_logprobs, token_logprobs_from_hidden
 
         cfg = self.cfg
         B, S = ids.shape
+
+        def score(h, targets, first):
+            if shaping is None:
+                return token_logprobs_from_hidden(h, self.lm_head.weight, targets, temperature)
+            return shaped_token_logprobs(h, self.lm_head.weight, targets, temperature, first=first, **shaping)
+
         if tp_decode is not None:
             # tensor-parallel rollout: heads split over the group, KV caches of this rank's heads only
             if caches is None:
@@ -428,7 +437,7 @@ class MoELLM(nn.Module):
             h = rms_norm(x, self.norm, cfg.eps)
             if targets is not None:
                 tl = F.pad(targets, (0, pad))[:, tp.rank * Sl:(tp.rank + 1) * Sl]
-                lp = token_logprobs_from_hidden(h, self.lm_head.weight, tl, temperature)
+                lp = score(h, tl, tp.rank * Sl)
                 return gather_sequence(lp.unsqueeze(-1), tp.group)[:, :S, 0]
             if return_hidden:
                 return gather_sequence(h, tp.group)[:, :S]
@@ -438,7 +447,7 @@ class MoELLM(nn.Module):
             x = blk(x, cos, sin, None if caches is None else caches[i], pos0, self.ep)
         h = rms_norm(x, self.norm, cfg.eps)
         if targets is not None:
-            return token_logprobs_from_hidden(h, self.lm_head.weight, targets, temperature)
+            return score(h, targets, 0)
         if return_hidden:
             return h
         return self.lm_head(h).float()

@@ -25,7 +25,7 @@ from verl_omni_b200.utils.dataproto import DataProto
 from verl_omni_b200.workers.config.diffusion import DiffusionActorConfig
 from verl_omni_b200.workers.engine.base import ShardedEngine
 from verl_omni_b200.workers.reward.reward_manager import hash_token_reward
-from verl_omni_b200.workers.rollout.llm_rollout import LLMRolloutEngine
+from verl_omni_b200.workers.rollout.llm_rollout import LLMRolloutEngine, said_tokens
 
 
 class OmniGRPOTrainer:
@@ -40,7 +40,10 @@ class OmniGRPOTrainer:
         decodes through the stages and the update runs the 1F1B schedule over the micro-batches.
 
         ``rollout_kw``: further options of :class:`~verl_omni_b200.workers.rollout.llm_rollout.LLMRolloutEngine` (8-bit KV
-        cache, penalties)."""
+        cache, penalties, logit bias).  With penalties or a bias old and new log-probs are those of the shaped distribution,
+        which the responses are drawn from; a grammar mask is refused, training does not know it."""
+        if (rollout_kw or {}).get("allowed_tokens") is not None:
+            raise ValueError("allowed_tokens: the trainer cannot recompute log-probs under a grammar mask")
         torch.manual_seed(seed)
         self.pp_size = int(pp_size)
         if self.pp_size > 1 and tp_group is not None and D.world_size(tp_group) > 1:
@@ -150,8 +153,13 @@ class OmniGRPOTrainer:
         tgt = torch.zeros_like(ids[:, :-1])
         tgt[:, P - 1:] = ids[:, P:]
         af, ip = self._feats(data)
+        kw = {}
+        if self.rollout.shaping is not None:  # the distribution that the responses were drawn from
+            pad = data.batch.get("prompt_pad")
+            kw["shaping"] = dict(history=said_tokens(ids, pad.to(self.device) if pad is not None else None), prompt_len=P,
+                                 **self.rollout.shaping)
         lp = self.model(ids[:, :-1], audio_feats=af, image_patches=ip, targets=tgt,
-                        temperature=self.temperature)
+                        temperature=self.temperature, **kw)
         return lp[:, P - 1:]
 
     def _feats(self, data: DataProto):
