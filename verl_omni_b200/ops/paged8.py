@@ -305,8 +305,9 @@ class PagedKVCache8:
 class PagedBatch8:
     """The sequences of one batch: their block table and row counts on the device, shared by the layers' views.
 
-    ``max_len``: rows that the table covers (at least what is reserved).  While a batch is in use, only it appends to
-    its sequences."""
+    ``max_len``: rows that the table covers (at least what is reserved); it grows when more are needed, until a step has been
+    captured in a CUDA graph, which reads the table at its address: from then on more is a RuntimeError.  While a batch is in
+    use, only it appends to its sequences."""
 
     def __init__(self, cache: PagedKVCache8, sids: list[int], max_len: int = 0):
         if len(set(sids)) != len(sids):
@@ -319,6 +320,7 @@ class PagedBatch8:
         self.lens = torch.tensor(self.base, dtype=torch.int32, device=dev)  # rows when the batch was made
         self.pos = self.lens.clone()  # position of the next row in steps that read it on the device
         self.off = 0  # rows appended since
+        self.captured = False  # a CUDA graph holds the table's address
         self._seen = -1
         self._refresh()
 
@@ -327,6 +329,7 @@ class PagedBatch8:
             return
         blocks = [self.cache.blocks[s] for s in self.sids]
         if max(len(b) for b in blocks) > self.table.shape[1]:
+            self._fits(max(len(b) for b in blocks))
             self.table = torch.zeros(len(blocks), max(len(b) for b in blocks), dtype=torch.int32, device=self.table.device)
         t = torch.zeros(self.table.shape, dtype=torch.int32)
         for i, b in enumerate(blocks):
@@ -334,10 +337,20 @@ class PagedBatch8:
         self.table.copy_(t)
         self._seen = self.cache.version
 
+    def _fits(self, pages: int) -> None:
+        if self.captured and pages > self.table.shape[1]:
+            raise RuntimeError(f"the block table holds {self.table.shape[1]} pages a sequence and a captured step reads it: "
+                               f"make the batch with max_len for {pages}")
+
+    def _reserve(self, n: int) -> None:
+        c = self.cache
+        self._fits(max(max(len(c.blocks[s]), -(-(c.length[s] + n) // c.block)) for s in self.sids))  # before anything changes
+        c.reserve(self.sids, n)
+
     def grow(self, off: int) -> None:
         """The batch's sequences hold ``off`` rows more than when it was made (pages are reserved as needed)."""
         if off > self.off:
-            self.cache.reserve(self.sids, off - self.off)
+            self._reserve(off - self.off)
             for s in self.sids:
                 self.cache.length[s] += off - self.off
             self.off = off
@@ -345,7 +358,7 @@ class PagedBatch8:
 
     def reserve(self, n: int) -> None:
         """Pages for ``n`` rows more than now, so that later steps change no table."""
-        self.cache.reserve(self.sids, n)
+        self._reserve(n)
         self._refresh()
 
     def at(self, off: int) -> None:
@@ -384,7 +397,13 @@ class Paged8View:
     def append_at(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """One row per sequence at the batch's device position (nothing is read on the host: the step can be captured in
         a CUDA graph; :meth:`PagedBatch8.at` moves the position between replays)."""
+        self._note_capture()
         append_paged8(k, v, *self._pools, self.batch.table, self.batch.pos)
 
     def attend_at(self, q: torch.Tensor, scale: Optional[float] = None) -> torch.Tensor:
+        self._note_capture()
         return attend_paged8(q, *self._pools, self.batch.table, self.batch.pos, None, scale, 1)
+
+    def _note_capture(self) -> None:
+        if self.batch.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            self.batch.captured = True
