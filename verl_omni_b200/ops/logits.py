@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import Optional, Union
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 Param = Union[float, torch.Tensor]
 
@@ -113,6 +114,7 @@ class _ProcessLogits(torch.autograd.Function):
         return _ext().process_logits(x, None, *args)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         x, *ts = ctx.saved_tensors
         it = iter(ts)
@@ -131,12 +133,14 @@ def process_logits(x: torch.Tensor, history: Optional[torch.Tensor] = None, lens
     (training: every position of a sequence has its own ``lens``).  ``repetition``, ``presence``, ``frequency``:
     numbers or fp32 ``[R]``.  ``bias`` fp32 ``[V]`` or ``[R, V]``; ``allowed`` int32 bitmask ``[R or 1, ceil(V / 32)]``
     (:func:`pack_allowed`).  A row whose mask allows nothing is ``-inf`` throughout.  The gradient is that of x; the
-    other arguments are constants."""
+    other arguments are constants.  On the GPU there is a first derivative in reverse mode, others are refused."""
     for t in (bias, repetition, presence, frequency):
         if isinstance(t, torch.Tensor) and t.requires_grad:
             raise ValueError("process_logits differentiates the logits only: detach bias and penalties")
     if not x.is_cuda:
         return process_logits_reference(x, history, lens, prompt_lens, rows, repetition, presence, frequency, bias, allowed)
+    if unpack_dual(x).tangent is not None:
+        raise ValueError("process_logits has no forward-mode derivative on the GPU")
     args = (history, lens, prompt_lens, rows, *_split(repetition), *_split(presence), *_split(frequency), bias, allowed)
     if x.requires_grad and torch.is_grad_enabled():
         return _ProcessLogits.apply(x, args)

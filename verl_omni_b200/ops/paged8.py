@@ -22,6 +22,7 @@ import math
 from typing import Optional, Sequence, Union
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 E4M3 = torch.float8_e4m3fn
 E4M3_MAX = 448.0
@@ -152,6 +153,8 @@ def attend_paged8(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k
     Inference only (no gradient).  Waits inside the kernels are bounded: :func:`raise_on_timeout` tells whether one ran out."""
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError("attention over the 8-bit cache has no backward: call it under torch.no_grad()")
+    if unpack_dual(q).tangent is not None:
+        raise ValueError("attention over the 8-bit cache has no forward-mode derivative")
     if not q.is_cuda:
         return attend_paged8_reference(q, k_pool, v_pool, k_scale, v_scale, block_table, lens, q_lens, scale, len_add)
     return _ext().paged8_attend(q, k_pool, v_pool, k_scale, v_scale, block_table, lens, q_lens,
