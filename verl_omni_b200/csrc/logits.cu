@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "per_device.h"
 
 namespace vo {
 namespace {
@@ -354,9 +355,8 @@ __global__ void __launch_bounds__(kThreads, 2) logits_kernel(const LogitArgs a) 
 template <typename T, bool BWD, bool ALIGNED, bool LONG>
 void launch(const LogitArgs& a) {
   constexpr int kMost = LONG ? kPartBytes / (int)sizeof(T) * 4 : (2 * 2 * kStaged + 2 * kStaged) * 4;
-  static const cudaError_t set =
-      cudaFuncSetAttribute(logits_kernel<T, BWD, ALIGNED, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-  VO_CUDA_OK(set);
+  static PerDevice once;
+  VO_CUDA_OK(once([] { return cudaFuncSetAttribute(logits_kernel<T, BWD, ALIGNED, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost); }));
   const int smem = !a.hist ? 0 : LONG ? kMost : (2 * table_size(a.L) + 2 * a.L) * 4;
   const int most = 2 * num_sms();
   const int64_t R = a.total / a.parts;

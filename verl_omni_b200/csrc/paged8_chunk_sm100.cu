@@ -23,6 +23,7 @@
 #include "dcheck.cuh"
 #include "paged8.cuh"
 #include "paged8_tc.h"
+#include "per_device.h"
 #include "tc8.cuh"
 
 namespace vo {
@@ -729,8 +730,9 @@ __global__ void __launch_bounds__(256) merge8_kernel(const __grid_constant__ Par
 
 template <int HD>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, cudaStream_t stream, int* launches) {
-  static const cudaError_t set = cudaFuncSetAttribute(chunk8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES);
-  if (set != cudaSuccess) return (int)set;
+  static PerDevice once;
+  cudaError_t e = once([] { return cudaFuncSetAttribute(chunk8_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::BYTES); });
+  if (e != cudaSuccess) return (int)e;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -741,7 +743,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G,
   cfg.gridDim = dim3(G);
   cfg.blockDim = dim3(NTHREADS);
   cfg.dynamicSmemBytes = Cfg<HD>::BYTES;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, chunk8_kernel<HD>, mk, mv, p);
+  e = cudaLaunchKernelEx(&cfg, chunk8_kernel<HD>, mk, mv, p);
   if (e != cudaSuccess) return (int)e;
   ++*launches;
   if (G == 1) return 0;

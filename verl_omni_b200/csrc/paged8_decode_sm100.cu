@@ -26,6 +26,7 @@
 #include "dcheck.cuh"
 #include "paged8.cuh"
 #include "paged8_tc.h"
+#include "per_device.h"
 #include "tc8.cuh"
 
 namespace vo {
@@ -693,9 +694,11 @@ __global__ void __launch_bounds__(256) combine8_kernel(const AttendArgs a, const
 
 template <int HD, int NR, bool CAUSAL>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G, cudaStream_t stream, int* launches) {
-  static const cudaError_t set =
-      cudaFuncSetAttribute(decode8_kernel<HD, NR, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD, NR>::BYTES);
-  if (set != cudaSuccess) return (int)set;
+  static PerDevice once;
+  cudaError_t e = once([] {
+    return cudaFuncSetAttribute(decode8_kernel<HD, NR, CAUSAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD, NR>::BYTES);
+  });
+  if (e != cudaSuccess) return (int)e;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -706,7 +709,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Params& p, int G,
   cfg.gridDim = dim3(G);
   cfg.blockDim = dim3(NTHREADS);
   cfg.dynamicSmemBytes = Cfg<HD, NR>::BYTES;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, decode8_kernel<HD, NR, CAUSAL>, mk, mv, p);
+  e = cudaLaunchKernelEx(&cfg, decode8_kernel<HD, NR, CAUSAL>, mk, mv, p);
   if (e != cudaSuccess) return (int)e;
   ++*launches;
   if (G == 1) return 0;
