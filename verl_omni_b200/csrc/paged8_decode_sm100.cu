@@ -61,7 +61,8 @@ struct Cfg {
   static constexpr int TV_OFF = SC_OFF + SV * 2 * kMaxBlocksPerTile * 4;       // per V tile: largest v scale, whether a page is missing, 2^8 / the former
   static constexpr int RED_OFF = TV_OFF + SV * 16;                             // [2][4][MAXR] warp maxima
   static constexpr int QS_OFF = RED_OFF + 2 * 4 * MAXR * 4;                    // [2][MAXR] row factors
-  static constexpr int BAR_OFF = QS_OFF + 2 * MAXR * 4;
+  static constexpr int FOLD_OFF = QS_OFF + 2 * MAXR * 4;                       // [4][2][2][MAXR] a warp's row factors of the fold
+  static constexpr int BAR_OFF = FOLD_OFF + 4 * 2 * 2 * MAXR * 4;
   static constexpr int NBARS = 2 * SK + 2 * SV + 11;
   static constexpr int START_OFF = BAR_OFF + NBARS * 8;  // tmem slot, abort flag, start item, scan sums
   static constexpr int BYTES = START_OFF + 96 + 1024;
@@ -393,6 +394,10 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     };
     const uint32_t trow = tmem + ((uint32_t)(warp * 32) << 16);
     const int blk = min(a.block, TK), my_blk = tid / blk;
+    // row factors of a tile's fold, by its parity, a copy per warp (they are the same in all threads, and registers are short): what
+    // is there already shrinks by alpha where the maximum grew, the tile's output by down where its reference lies below it
+    float* alpha = reinterpret_cast<float*>(sm + C::FOLD_OFF) + warp * 4 * MAXR;
+    float* down = alpha + 2 * MAXR;
     int seg = 0, it = 0;
     if (ntot > 0) {
       fetch_q(w.b, w.kh);
@@ -401,19 +406,16 @@ __global__ void __launch_bounds__(NTHREADS, 2)
     while (it < ntot) {
       const int nseg = min(w.nt - w.tile, ntot - it), nq = p8::seq_q(a, w.b);
       const bool from_start = w.tile == 0, whole = from_start && nseg == w.nt;
-      float m[NR], lpart[NR], acc[NR], alpha[NR], qf[NR];
+      float m[NR], lpart[NR], acc[NR], qf[NR];
       int lim[CAUSAL ? NR : 1];
-      float vfac = 0.f;  // of the tile that is folded next, with alpha where its maximum grew
-      bool rescale = false, far = false;
-      uint32_t down[NR / 4];  // log2 that its reference lies below the running maximum, a byte per row; where far
-      auto shift = [](const uint32_t* d, int h) { return (int)((d[h / 4] >> (h % 4 * 8)) & 0xff); };
+      float vfac = 0.f;  // of the tile that is folded next
+      bool rescale = false, far = false;  // and whether it has row factors
       int nan_at = 0x7fffffff;  // first key whose value in this thread's column is NaN (tiles that a row sees partly)
       compute_sync();           // row factors of this item are written
 #pragma unroll
       for (int h = 0; h < NR; ++h) {
         m[h] = -INFINITY;
         lpart[h] = acc[h] = 0.f;
-        alpha[h] = 1.f;
         qf[h] = qsc[(seg & 1) * MAXR + h];
         if (CAUSAL) {
           const int s = h / a.rep;
@@ -433,12 +435,19 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         wait_ld();
         fence_before();
         mbar_arrive(&o_empty[sb]);
+        if (rescale) {
 #pragma unroll
-        for (int h = 0; h < NR; ++h) {
-          if (rescale) acc[h] *= alpha[h];
-          const float o = fmaf(__uint_as_float(r[NP + h]), 1.f / kPLow, __uint_as_float(r[h]));
-          acc[h] = fmaf(o, far ? vfac * p8::pow2(-shift(down, h)) : vfac, acc[h]);
+          for (int h = 0; h < NR; ++h) acc[h] *= alpha[sb * MAXR + h];
         }
+        if (far) {
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const float f = down[sb * MAXR + h];
+            r[h] = __float_as_uint(__uint_as_float(r[h]) * f), r[NP + h] = __float_as_uint(__uint_as_float(r[NP + h]) * f);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < NR; ++h) acc[h] = fmaf(fmaf(__uint_as_float(r[NP + h]), 1.f / kPLow, __uint_as_float(r[h])), vfac, acc[h]);
       };
       const Walk cur = w;
       next_item(w, a);
@@ -495,44 +504,20 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         }
 #pragma unroll
         for (int h = 0; h < NR; ++h) grown = grown || mx[h] > m[h];
-        float alpha_now[NR];
         if (grown) {  // the same in all threads; rare once a sequence is under way
 #pragma unroll
           for (int h = 0; h < NR; ++h) {
-            const float mn = fmaxf(m[h], mx[h]);
-            alpha_now[h] = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
-            lpart[h] *= alpha_now[h];
+            const float mn = fmaxf(m[h], mx[h]), al = mn == -INFINITY ? 1.f : ex2(m[h] - mn);
+            lpart[h] *= al;
             m[h] = mn;
-          }
-        }
-        bool far_now = false;  // the same in all threads, too
-#pragma unroll
-        for (int h = 0; h < NR; ++h) far_now = far_now || m[h] - mx[h] > kFar;
-        uint32_t down_now[NR / 4];
-        if (far_now) {
-#pragma unroll
-          for (int h = 0; h < NR; ++h) {
-            const float gap = m[h] - mx[h];  // no key of the tile seen: infinite, no weight either; none so far: NaN
-            const uint32_t d = gap > kFar ? (uint32_t)fminf(gap, 126.f) : 0;
-            down_now[h / 4] = h % 4 ? down_now[h / 4] | d << (h % 4 * 8) : d;
+            if (lane == 0) alpha[sb * MAXR + h] = al;
           }
         }
         uint8_t* pb = sm + C::P_OFF + sb * NB * TK;
         const int prow = tid & 15, pcol = tid >> 4;
-#pragma unroll
-        for (int h = 0; h < NR; h += 2) {
-          float e0, e1;
-          if (full) {  // m is finite, or the scores are NaN
-            e0 = ex2(s[h] - m[h]), e1 = ex2(s[h + 1] - m[h + 1]);
-          } else {
-            e0 = s[h] == -INFINITY ? 0.f : ex2(s[h] - m[h]);
-            e1 = s[h + 1] == -INFINITY ? 0.f : ex2(s[h + 1] - m[h + 1]);
-          }
-          lpart[h] += e0;
-          lpart[h + 1] += e1;
-          if (far_now) e0 *= p8::pow2(shift(down_now, h)), e1 *= p8::pow2(shift(down_now, h + 1));
-          // p to 8 bits: the nearest e4m3 number and the nearest one to what is left (f16 between: 11 bits)
-          const __half2 p16 = __floats2half2_rn(e0 * vr, e1 * vr);
+        // p to 8 bits: the nearest e4m3 number and the nearest one to what is left (f16 between: 11 bits)
+        auto emit = [&](int h, float p0, float p1) {
+          const __half2 p16 = __floats2half2_rn(p0, p1);
           const __nv_fp8x2_storage_t hi = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&p16), __NV_SATFINITE, __NV_E4M3);
           const __half2_raw back = __nv_cvt_fp8x2_to_halfraw2(hi, __NV_E4M3);
           const __half2 rest = __hmul2(__hsub2(p16, *reinterpret_cast<const __half2*>(&back)), __float2half2_rn(kPLow));
@@ -543,7 +528,27 @@ __global__ void __launch_bounds__(NTHREADS, 2)
           d1[0] = (uint8_t)(hi >> 8);
           d0[NP * TK] = (uint8_t)lo2;
           d1[NP * TK] = (uint8_t)(lo2 >> 8);
+        };
+        bool far_now = false;  // the same in all threads, too
+#pragma unroll
+        for (int h = 0; h < NR; ++h) far_now = far_now || m[h] - mx[h] > kFar;
+#pragma unroll
+        for (int h = 0; h < NR; ++h) {
+          // in a full tile m is finite, or the scores are NaN
+          s[h] = full || s[h] != -INFINITY ? ex2(s[h] - m[h]) : 0.f;
+          lpart[h] += s[h];
         }
+        if (far_now) {
+#pragma unroll
+          for (int h = 0; h < NR; ++h) {
+            const float gap = m[h] - mx[h];  // no key of the tile seen: infinite, no weight either; none so far: NaN
+            const float f = p8::pow2(gap > kFar ? -(int)fminf(gap, 126.f) : 0);
+            s[h] *= inv_pow2(f);
+            if (lane == 0) down[sb * MAXR + h] = f;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < NR; h += 2) emit(h, s[h] * vr, s[h + 1] * vr);
         if (!full) {
           uint8_t* vt = sm + C::V_OFF + st * C::KV;
           if (!there) {  // rows that hold nothing: zero, so that 0 * garbage stays 0
@@ -567,15 +572,7 @@ __global__ void __launch_bounds__(NTHREADS, 2)
         if (last_q) load_q((seg & 1) ^ 1);  // scores of this item are all read
         if (j > 0) fold(i - 1);
         rescale = grown;
-        if (grown) {
-#pragma unroll
-          for (int h = 0; h < NR; ++h) alpha[h] = alpha_now[h];
-        }
         far = far_now;
-        if (far_now) {
-#pragma unroll
-          for (int k = 0; k < NR / 4; ++k) down[k] = down_now[k];
-        }
         vfac = tv.x * (1.f / kPOne);
       }
       fold(it + nseg - 1);
