@@ -13,7 +13,7 @@
 // evenly over one CTA per SM; causal items are as long as their last row's reach; cut items are merged in key order.
 // Warps 0-3 and 4-7: softmax and output of row tile 0 and 1 (thread = row); 8-11 and 12-14: K and V pages -> f16 tiles in
 // shared memory (the codes come by TMA, a tile ahead); 15: tensor-memory allocation, MMA issue.
-// Measured (B200): 4 x 512 tokens on 8000 rows, 32 query and 4 KV heads of 128: 370 us, 702 TFLOP/s.  What bounds it is the
+// Measured (B200): 4 x 512 tokens on 8000 rows, 32 query and 4 KV heads of 128: 366 us, 710 TFLOP/s.  What bounds it is the
 // chain of a tile (scores, softmax, second product): leaving out the stores of the conversion, the exponentials or half of
 // either product gained 3 to 9 % each.  64-key tiles with the scores a tile ahead: 513 us.
 // The loops are kept short (few unrolled copies): five roles run at once, and with everything unrolled the warps mostly

@@ -18,9 +18,10 @@
 // there are tiles at most), so ragged lengths balance and a long single sequence fills the GPU.  An item inside one CTA
 // is finished there; one cut by a border leaves (maximum, sum, output) partials that the combine kernel merges in
 // the order of the keys, so results do not depend on timing.
-// Measured (B200, 8 query heads per KV head): 64 sequences x 4096 rows, 4 KV heads of 128, pages of 128: 56.7 us; its bytes
-// alone take 41 us.  Time grows by 7.0 TB/s with the rows over about 20 us (fill, item changes, merge).  K and V in one
-// ring: 57 us; a second softmax group taking every other tile: 65 us.
+// Measured (B200, 8 query heads per KV head): 64 sequences x 4096 rows, 4 KV heads of 128, pages of 128: 56.4 us, the same with
+// one key far above the others; its bytes alone take 41 us.  16 heads per KV head: 90 us; 2 tokens x 8 heads: 125 us.  Time grows by
+// 7.0 TB/s with the rows over about 20 us (fill, item changes, merge).  Before small weights were kept 54.6 us; against that K and
+// V in one ring took 57, a second softmax group taking every other tile 65 us.
 // Warps 0-3: softmax (thread = key) and output (thread = head-dim column); 4: TMA producer, page ids read two tiles and
 // scales one tile ahead; 5: tensor-memory allocation, MMA issue (scores one tile ahead of the softmax).
 #include "dcheck.cuh"
